@@ -192,6 +192,54 @@ SNNTC_API int snntc_sgdm_step(float* w, const float* g, float* vel, size_t n, fl
                               float grad_scale, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
+ * The two ends of a network on tokens. None of these has a counterpart in the reference. Sizes N, V and R are 64-bit and
+ * limited to 2^31-1 (V: 2^31-2); tensors may have more elements than that. Workspaces are 256-byte aligned.
+ *
+ * snntc_embedding_forward   y[N,D]: row t is scale * table[ids[t],:], or exp(scale * table[ids[t],:]) where `spikes` is not 0
+ *                    (rows of spike times, encoded as snntc_encode does with one_minus = 0). Where ids[t] == padding or is
+ *                    outside [0, V): no_spike in all D places, and table is not read. ids: int32 or int64 (id_bytes 4 or 8).
+ *                    N = 0 is a no-op.
+ * snntc_embedding_backward  dtable[V,D] is written in full: the gradient of the table for the upstream gradient g[N,D], each row
+ *                    summed over its tokens in the order of t (zeros where no token names it). `table` is read only where
+ *                    `spikes` is not 0 and may be null otherwise. The same bits every run.
+ *
+ * For the losses z[R,J] are spike values (logits are -z) and labels[R] int64; a row whose label is outside [0, J) does not count:
+ * its logits are not read, its log-probability is 0 and its gradient 0. stats_2R (R pairs of floats) receives what the backward
+ * needs of every row's softmax, factor (R floats) dloss / d(log-probability of the row's label).
+ * snntc_label_logp_forward  logp[r] = log softmax(-z[r,:])[labels[r]]; stats_2R may be null.
+ * snntc_choice_backward     dz[r,:] = factor[r] * *gout * (softmax(-z[r,:]) - onehot(labels[r])); gout (device) may be null: 1.
+ *                    Serves all three losses; for snntc_label_logp_forward factor is the upstream gradient.
+ * snntc_policy_loss  the mean over the rows that count of -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * k with
+ *                    r = exp(lp - old_logp), A = advantage, k = exp(ref_logp - lp) - (ref_logp - lp) - 1. *loss and
+ *                    kl_and_clipped[2] (mean k; share of rows whose ratio was clipped) are written; 0 where no row counts.
+ *                    ref_logp may be null where kl_coef is 0.
+ * snntc_preference_loss  texts 0..P-1 are preferred to texts P..2P-1: text s is rows [starts[s], starts[s+1]) (2P+1 ascending
+ *                    offsets, device; they are held to [0, R]) or, where starts is null, the s-th of 2P equal parts of the rows.
+ *                    margins[k] = beta * ((S_k - ref_k) - (S_{P+k} - ref_{P+k})) with S the sum of a text's log-probabilities
+ *                    (ref_logp[2P] may be null: 0); *loss = mean_k of -(1 - smoothing) log sigma(margins[k])
+ *                    - smoothing log sigma(-margins[k]). Rows of no text have no part in it.
+ */
+SNNTC_API int snntc_embedding_forward(const void* ids, int id_bytes, const float* table, float* y, long long N, long long V, int D,
+                                      float scale, int spikes, long long padding, float no_spike, void* stream);
+SNNTC_API size_t snntc_embedding_backward_workspace_bytes(long long N, long long V, int D);
+SNNTC_API int snntc_embedding_backward(const void* ids, int id_bytes, const float* g, const float* table, float* dtable, long long N,
+                                       long long V, int D, float scale, int spikes, long long padding, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+SNNTC_API int snntc_label_logp_forward(const float* z, const long long* labels, float* logp, float* stats_2R, long long R, int J,
+                                       void* stream);
+SNNTC_API int snntc_choice_backward(const float* z, const long long* labels, const float* stats_2R, const float* factor,
+                                    const float* gout, float* dz, long long R, int J, void* stream);
+SNNTC_API size_t snntc_policy_loss_workspace_bytes(long long R);
+SNNTC_API int snntc_policy_loss(const float* z, const long long* labels, const float* old_logp, const float* advantage,
+                                const float* ref_logp, float* loss, float* kl_and_clipped, float* stats_2R, float* factor,
+                                long long R, int J, double clip_low, double clip_high, double kl_coef, void* workspace,
+                                size_t workspace_bytes, void* stream);
+SNNTC_API size_t snntc_preference_loss_workspace_bytes(long long R, int P);
+SNNTC_API int snntc_preference_loss(const float* z, const long long* labels, const long long* starts, const float* ref_logp,
+                                    float* loss, float* margins, float* stats_2R, float* factor, long long R, int J, int P,
+                                    double beta, double smoothing, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
  * SnnFcGrad without a caller workspace. This entry point has no counterpart in the reference.
  *
  * For callers that have no way to allocate device memory when the dense backward runs (an operator

@@ -116,6 +116,36 @@ class SNN_conv(torch.nn.Module):
         return (self.weight ** 2).mean()
 
 
+class SNN_embedding(torch.nn.Module):
+    """The input layer of a network on tokens, which the reference, fed with pixels, does not have: integer ids of any shape
+    to spike values [..., out_size] -- exp(scale * row of spike times), or with spikes=False scale * row. A padding token
+    (padding_idx, or any id outside the table) never spikes: its values are MAX_SPIKE_TIME. Ids [B,L] feed SNN_dense
+    through a Flatten; ids [B,H,W] (H = 1 for texts) give the NHWC input of SNN_conv."""
+
+    def __init__(self, num_tokens=1, out_size=1, scale=1.0, padding_idx=None, spikes=True, MAX_SPIKE_TIME=1e5, weight=None,
+                 name=None):
+        super().__init__()
+        self.num_tokens = num_tokens
+        self.out_size = out_size
+        self.scale = float(scale)
+        self.padding_idx = padding_idx
+        self.spikes = bool(spikes)
+        self.MAX_SPIKE_TIME = float(MAX_SPIKE_TIME)
+        if weight is None:   # spike times in [0, 1), what the encoding of pixels gives
+            weight = np.random.rand(num_tokens, out_size).astype(np.float32)
+        weight = _to_weight(weight)
+        self.name = name if name is not None else "embkernel"
+        if tuple(weight.shape) != (num_tokens, out_size):
+            raise ValueError("weight must have shape [%d, %d], got %s" % (num_tokens, out_size, tuple(weight.shape)))
+        self.weight = torch.nn.Parameter(weight)
+        self.grad_sink = None
+
+    def forward(self, ids):
+        return ops.snn_embedding(ids, self.weight, self.scale, self.padding_idx, self.spikes, self.MAX_SPIKE_TIME, self.grad_sink)
+
+    call = forward
+
+
 def _same_pad_nhwc(input, Kh, Kw, Sh, Sw, value):
     B, H, W, C = input.shape
     th = (math.ceil(H / Sh) - 1) * Sh + Kh - H

@@ -12,6 +12,7 @@ MEASURE_LIB_PATH = os.path.join(_HERE, "libsnntc_b200_measure.so")
 # every symbol include/snntc_b200.h declares: (restype, argtypes)
 _F = ctypes.c_void_p  # device/host float pointers travel as integers
 _INT = ctypes.c_int
+_LL = ctypes.c_longlong
 _SZ = ctypes.c_size_t
 SYMBOLS = {
     "snntc_status_string": (ctypes.c_char_p, [_INT]),
@@ -47,6 +48,15 @@ SYMBOLS = {
     "snntc_weight_cost": (_INT, [_F, _F, _F, _INT, _INT, ctypes.c_float, ctypes.c_float, _F, _SZ, _F]),
     "snntc_adam_step": (_INT, [_F, _F, _F, _F, _SZ] + [ctypes.c_float] * 5 + [_F, _F]),
     "snntc_sgdm_step": (_INT, [_F, _F, _F, _SZ] + [ctypes.c_float] * 3 + [_F]),
+    "snntc_embedding_forward": (_INT, [_F, _INT, _F, _F, _LL, _LL, _INT, ctypes.c_float, _INT, _LL, ctypes.c_float, _F]),
+    "snntc_embedding_backward_workspace_bytes": (_SZ, [_LL, _LL, _INT]),
+    "snntc_embedding_backward": (_INT, [_F, _INT, _F, _F, _F, _LL, _LL, _INT, ctypes.c_float, _INT, _LL, _F, _SZ, _F]),
+    "snntc_label_logp_forward": (_INT, [_F] * 4 + [_LL, _INT, _F]),
+    "snntc_choice_backward": (_INT, [_F] * 6 + [_LL, _INT, _F]),
+    "snntc_policy_loss_workspace_bytes": (_SZ, [_LL]),
+    "snntc_policy_loss": (_INT, [_F] * 9 + [_LL, _INT] + [ctypes.c_double] * 3 + [_F, _SZ, _F]),
+    "snntc_preference_loss_workspace_bytes": (_SZ, [_LL, _INT]),
+    "snntc_preference_loss": (_INT, [_F] * 8 + [_LL, _INT, _INT] + [ctypes.c_double] * 2 + [_F, _SZ, _F]),
 }
 # exported by the measurement build only (include/snntc_b200.h, #ifdef SNNTC_MEASURE)
 MEASURE_SYMBOLS = {

@@ -25,7 +25,7 @@ SOURCES = ["snntc_forward.cu", "snntc_sort.cu", "snntc_walk_ring.cu", "snntc_wal
            "snntc_lists.cu", "snntc_backward.cu", "snntc_bwd_dense.cu",
            "snntc_dw_skip.cu", "snntc_dw_tma.cu", "snntc_dx_sparse.cu", "snntc_dx_few.cu",
            "snntc_pool.cu",
-           "snntc_noalloc.cu", "snntc_train.cu", "snntc_api.cu"]
+           "snntc_noalloc.cu", "snntc_train.cu", "snntc_embed.cu", "snntc_choice.cu", "snntc_api.cu"]
 NATIVE = os.path.join(HERE, "_native" + sysconfig.get_config_var("EXT_SUFFIX"))
 NATIVE_SOURCE = os.path.join(CSRC, "snntc_torch.cpp")
 API_SOURCE = "snntc_api.cu"   # the only file that reads SNNTC_MEASURE

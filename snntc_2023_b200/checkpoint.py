@@ -14,18 +14,20 @@ line on the reference side:
 import numpy as np
 import torch
 
-from .SNN_TC_Modules import SNN_conv, SNN_dense
+from .SNN_TC_Modules import SNN_conv, SNN_dense, SNN_embedding
 
 
 def keras_names(model):
     """[(variable name, layer)] for the weighted layers of `model` in construction (module) order."""
     out = []
-    counts = {"snn_dense": 0, "snn_conv": 0}
+    counts = {"snn_dense": 0, "snn_conv": 0, "snn_embedding": 0}
     for layer in model.modules():
         if isinstance(layer, SNN_dense):
             base, kernel = "snn_dense", "fckernel"
         elif isinstance(layer, SNN_conv):
             base, kernel = "snn_conv", "convkernel"
+        elif isinstance(layer, SNN_embedding):   # no counterpart in the reference; named in its manner
+            base, kernel = "snn_embedding", "embkernel"
         else:
             continue
         n = counts[base]

@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/graph_task.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <mutex>
 
@@ -544,6 +545,262 @@ Tensor constraint_cost(const std::vector<Tensor>& weights, double K, double K2) 
   return CostFunction::apply(at::TensorList(weights), s);
 }
 
+// ------------------------------------------------------------------------------------------------ embedding, losses on choices
+// The nodes below compute gradients by kernels that nothing differentiates: asked for a graph of the gradient they refuse, instead
+// of handing out one that is a constant. And a leaf whose gradient accumulator lives on another stream -- an eager graph of the
+// same leaf is still alive -- would draw that stream into a capture under way, which ends the process: refused as well, before
+// autograd gets there.
+void check_backward(const Tensor& on, const char* what) {
+  if (at::GradMode::is_enabled()) throw SnntcFailure(std::string(what) + ": the gradient cannot be differentiated again (create_graph)");
+  const auto current = at::cuda::getCurrentCUDAStream(on.get_device());
+  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(current.stream(), &capturing) != cudaSuccess || capturing == cudaStreamCaptureStatusNone) return;
+  for (const torch::autograd::Edge& edge : torch::autograd::get_current_node()->next_edges()) {
+    auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
+    if (leaf == nullptr) continue;
+    const auto stream = leaf->stream();
+    if (stream.has_value() && *stream != current.unwrap())
+      throw SnntcFailure(std::string(what) + ": a backward pass is being captured while a graph of the same leaf that was built on "
+                         "another stream is alive; release that graph (its outputs) before the capture");
+  }
+}
+
+Tensor on_device(const Tensor& t, const Tensor& like, const char* name) {
+  TORCH_CHECK_VALUE(t.device() == like.device(), name, " must be on ", like.device(), ", got ", t.device());
+  return t;
+}
+
+struct EmbedState : torch::CustomClassHolder {
+  double scale, no_spike;
+  bool spikes;
+  int64_t padding, V, D;
+  Tensor sink;      // where dE goes instead of into autograd: a slice of the flat gradient bucket
+};
+
+const void* id_ptr(const Tensor& ids, int* bytes) {
+  *bytes = (int)ids.element_size();
+  return ids.data_ptr();
+}
+
+Tensor embed_forward_call(const Tensor& w, const Tensor& ids, const EmbedState& s) {
+  const c10::cuda::CUDAGuard guard(w.device());
+  auto shape = ids.sizes().vec();
+  shape.push_back(s.D);
+  const Tensor y = empty_like_dev(shape, w);
+  int bytes;
+  const void* p = id_ptr(ids, &bytes);
+  check(snntc_embedding_forward(p, bytes, ptr(w), ptr(y), ids.numel(), s.V, to_int(s.D, "embedding"), (float)s.scale, s.spikes, s.padding,
+                                (float)s.no_spike, stream_of(w)), "embedding");
+  return y;
+}
+
+struct EmbedFunction : torch::autograd::Function<EmbedFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& W, const Tensor& ids, c10::intrusive_ptr<EmbedState> s) {
+    const Tensor w = W.contiguous();
+    ctx->saved_data["call"] = c10::IValue::make_capsule(s);
+    if (s->spikes) ctx->save_for_backward({ids, w});
+    else ctx->save_for_backward({ids});
+    return embed_forward_call(w, ids, *s);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = c10::static_intrusive_pointer_cast<EmbedState>(ctx->saved_data["call"].toCapsule());
+    const auto saved = ctx->get_saved_variables();
+    const Tensor& ids = saved[0];
+    const Tensor g = as_cuda_f32(grads[0], "grad");
+    const c10::cuda::CUDAGuard guard(g.device());
+    if (!s->sink.defined()) check_backward(g, "embedding");
+    const Tensor dw = s->sink.defined() ? s->sink : empty_like_dev({s->V, s->D}, g);
+    const int D = to_int(s->D, "embedding");
+    const size_t bytes = snntc_embedding_backward_workspace_bytes(ids.numel(), s->V, D);
+    const Tensor ws = workspace(bytes, g);
+    int id_bytes;
+    const void* p = id_ptr(ids, &id_bytes);
+    check(snntc_embedding_backward(p, id_bytes, ptr(g), s->spikes ? ptr(saved[1]) : nullptr, ptr(dw), ids.numel(), s->V, D, (float)s->scale,
+                                   s->spikes, s->padding, ws.data_ptr(), bytes, stream_of(g)), "embedding");
+    return {s->sink.defined() ? Tensor() : dw, Tensor(), Tensor()};
+  }
+};
+
+Tensor embedding(const Tensor& ids_in, const Tensor& W, double scale, bool spikes, std::optional<int64_t> padding, double no_spike,
+                 const std::optional<Tensor>& sink) {
+  const Tensor w = as_cuda_f32(W, "weight");
+  TORCH_CHECK_VALUE(w.dim() == 2 && w.size(0) > 0 && w.size(1) > 0, "embedding expects a weight [tokens, dimensions]");
+  TORCH_CHECK_VALUE(ids_in.scalar_type() == at::kLong || ids_in.scalar_type() == at::kInt, "ids must be int32 or int64, got ", ids_in.scalar_type());
+  const Tensor ids = on_device(ids_in, w, "ids").contiguous();
+  TORCH_CHECK_VALUE(std::isfinite(scale), "embedding: scale must be finite");
+  auto s = c10::make_intrusive<EmbedState>();
+  s->scale = scale;
+  s->no_spike = no_spike;
+  s->spikes = spikes;
+  s->padding = padding.value_or(-1);      // an id that no table has
+  s->V = w.size(0);
+  s->D = w.size(1);
+  if (!(at::GradMode::is_enabled() && W.requires_grad())) return embed_forward_call(w, ids, *s);
+  if (sink.has_value()) {
+    s->sink = *sink;
+    TORCH_CHECK_VALUE(s->sink.device() == w.device() && s->sink.scalar_type() == at::kFloat && s->sink.is_contiguous() &&
+                      s->sink.sizes() == w.sizes(), "embedding: grad_sink must be a contiguous float32 tensor of the weight's shape");
+  }
+  return EmbedFunction::apply(W, ids, s);
+}
+
+// Rows of a loss on choices: z[R,J], labels[R] and one number per row for the rest.
+struct Rows {
+  Tensor z, label;
+  int64_t R;
+  int J;
+};
+Rows choice_rows(const Tensor& logit, const Tensor& label, const char* what) {
+  Rows r;
+  r.z = as_cuda_f32(logit.detach(), "logit");     // (the version counter is shared: a change in place before the backward is noticed)
+  TORCH_CHECK_VALUE(logit.dim() >= 2 && logit.sizes().slice(0, logit.dim() - 1) == label.sizes(), what,
+                    " expects logit[..., classes] and label[...] with the same leading dimensions, got ", logit.sizes(), " and ", label.sizes());
+  TORCH_CHECK_VALUE(at::isIntegralType(label.scalar_type(), false), "label must hold integers, got ", label.scalar_type());
+  r.label = label.to(logit.device(), at::kLong).contiguous();
+  r.R = label.numel();
+  TORCH_CHECK_VALUE(r.R > 0 && logit.size(-1) > 0, what, " expects at least one row and one class");
+  r.J = to_int(logit.size(-1), what);
+  return r;
+}
+const long long* labels_of(const Tensor& t) { return (const long long*)t.data_ptr<int64_t>(); }
+
+Tensor constant(const Tensor& t, const Tensor& like, int64_t n, const char* name) {
+  const Tensor c = on_device(as_cuda_f32(t, name), like, name);
+  TORCH_CHECK_VALUE(c.numel() == n, name, " must hold ", n, " values, got ", c.numel());
+  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t.requires_grad()), name, " is a constant of the loss: detach it");
+  return c;
+}
+
+Tensor choice_backward(const Tensor& z, const Tensor& label, const Tensor& stats, const Tensor& factor, const Tensor& gout, const char* what) {
+  const c10::cuda::CUDAGuard guard(z.device());
+  const Tensor dz = empty_like_dev(z.sizes(), z);
+  check(snntc_choice_backward(ptr(z), labels_of(label), ptr(stats), ptr(factor), ptr(gout), ptr(dz), label.numel(), (int)z.size(-1), stream_of(z)),
+        what);
+  return dz;
+}
+
+Tensor label_logp_call(const Rows& r, const Tensor& stats) {
+  const c10::cuda::CUDAGuard guard(r.z.device());
+  const Tensor logp = empty_like_dev(r.label.sizes(), r.z);
+  check(snntc_label_logp_forward(ptr(r.z), labels_of(r.label), ptr(logp), ptr(stats), r.R, r.J, stream_of(r.z)), "label_log_probs");
+  return logp;
+}
+
+struct LabelLogpFunction : torch::autograd::Function<LabelLogpFunction> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& logit, const Tensor& label) {
+    const Rows r = choice_rows(logit, label, "label_log_probs");
+    const Tensor stats = empty_like_dev({r.R, 2}, r.z);
+    const Tensor logp = label_logp_call(r, stats);
+    ctx->save_for_backward({r.z, r.label, stats});
+    return logp;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    check_backward(saved[0], "label_log_probs");
+    const Tensor g = as_cuda_f32(grads[0], "grad");
+    return {choice_backward(saved[0], saved[1], saved[2], g, Tensor(), "label_log_probs"), Tensor()};
+  }
+};
+
+Tensor label_log_probs(const Tensor& logit, const Tensor& label) {
+  if (at::GradMode::is_enabled() && logit.requires_grad()) return LabelLogpFunction::apply(logit, label);
+  return label_logp_call(choice_rows(logit, label, "label_log_probs"), Tensor());
+}
+
+// What a loss over rows is called with besides the logits: constants, no gradient goes to them.
+struct ChoiceState : torch::CustomClassHolder {
+  Rows rows;
+  Tensor old_logp, advantage, ref_logp, starts;
+  double a, b, c;     // clip_low, clip_high, kl_coef; beta, label_smoothing
+  int P = 0;          // pairs; 0: a policy loss
+  const char* name() const { return P ? "preference_loss" : "policy_loss"; }
+};
+struct ChoiceLoss { Tensor loss, more, stats, factor; };   // more: [KL term, clipped] or the margins
+
+ChoiceLoss choice_loss_call(const ChoiceState& s) {
+  const Rows& r = s.rows;
+  const c10::cuda::CUDAGuard guard(r.z.device());
+  ChoiceLoss o;
+  o.loss = empty_like_dev({}, r.z);
+  o.more = empty_like_dev({s.P ? s.P : 2}, r.z);
+  o.stats = empty_like_dev({r.R, 2}, r.z);
+  o.factor = empty_like_dev({r.R}, r.z);
+  const size_t bytes = s.P ? snntc_preference_loss_workspace_bytes(r.R, s.P) : snntc_policy_loss_workspace_bytes(r.R);
+  const Tensor ws = workspace(bytes, r.z);
+  const int rc = s.P ? snntc_preference_loss(ptr(r.z), labels_of(r.label), s.starts.defined() ? labels_of(s.starts) : nullptr, ptr(s.ref_logp),
+                                             ptr(o.loss), ptr(o.more), ptr(o.stats), ptr(o.factor), r.R, r.J, s.P, s.a, s.b, ws.data_ptr(),
+                                             bytes, stream_of(r.z))
+                     : snntc_policy_loss(ptr(r.z), labels_of(r.label), ptr(s.old_logp), ptr(s.advantage), ptr(s.ref_logp), ptr(o.loss),
+                                         ptr(o.more), ptr(o.stats), ptr(o.factor), r.R, r.J, s.a, s.b, s.c, ws.data_ptr(), bytes, stream_of(r.z));
+  check(rc, s.name());
+  return o;
+}
+
+struct ChoiceLossFunction : torch::autograd::Function<ChoiceLossFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logit, c10::intrusive_ptr<ChoiceState> s) {
+    const ChoiceLoss o = choice_loss_call(*s);
+    ctx->save_for_backward({s->rows.z, s->rows.label, o.stats, o.factor});
+    ctx->saved_data["pairs"] = (int64_t)s->P;
+    ctx->mark_non_differentiable({o.more});
+    return {o.loss, o.more};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const char* what = ctx->saved_data["pairs"].toInt() ? "preference_loss" : "policy_loss";
+    check_backward(saved[0], what);
+    const Tensor g = as_cuda_f32(grads[0], "gradient of the loss");
+    return {choice_backward(saved[0], saved[1], saved[2], saved[3], g, what), Tensor()};
+  }
+};
+
+std::pair<Tensor, Tensor> choice_loss(const Tensor& logit, c10::intrusive_ptr<ChoiceState> s) {
+  if (at::GradMode::is_enabled() && logit.requires_grad()) {
+    auto r = ChoiceLossFunction::apply(logit, s);
+    return {r[0], r[1]};
+  }
+  const ChoiceLoss o = choice_loss_call(*s);
+  return {o.loss, o.more};
+}
+
+std::pair<Tensor, Tensor> policy_loss(const Tensor& logit, const Tensor& label, const Tensor& old_logp, const Tensor& advantage,
+                                      const std::optional<Tensor>& ref_logp, double clip_low, double clip_high, double kl_coef) {
+  TORCH_CHECK_VALUE(clip_low >= 0 && clip_low <= 1 && clip_high >= 0, "policy_loss: clip_low must be in [0, 1] and clip_high not negative");
+  TORCH_CHECK_VALUE(std::isfinite(kl_coef), "policy_loss: kl_coef must be finite");
+  TORCH_CHECK_VALUE(kl_coef == 0 || ref_logp.has_value(), "policy_loss: the KL term needs ref_logp");
+  auto s = c10::make_intrusive<ChoiceState>();
+  s->rows = choice_rows(logit, label, "policy_loss");
+  s->old_logp = constant(old_logp, s->rows.z, s->rows.R, "old_logp");
+  s->advantage = constant(advantage, s->rows.z, s->rows.R, "advantage");
+  if (ref_logp.has_value()) s->ref_logp = constant(*ref_logp, s->rows.z, s->rows.R, "ref_logp");
+  s->a = clip_low;
+  s->b = clip_high;
+  s->c = kl_coef;
+  return choice_loss(logit, s);
+}
+
+std::pair<Tensor, Tensor> preference_loss(const Tensor& logit, const Tensor& label, const std::optional<Tensor>& starts,
+                                          const std::optional<Tensor>& ref_logp, double beta, double smoothing) {
+  TORCH_CHECK_VALUE(std::isfinite(beta), "preference_loss: beta must be finite");
+  TORCH_CHECK_VALUE(smoothing >= 0 && smoothing <= 1, "preference_loss: label_smoothing must be in [0, 1]");
+  auto s = c10::make_intrusive<ChoiceState>();
+  s->rows = choice_rows(logit, label, "preference_loss");
+  int64_t texts;
+  if (starts.has_value()) {
+    TORCH_CHECK_VALUE(starts->dim() == 1 && starts->size(0) >= 3 && starts->size(0) % 2 == 1 && at::isIntegralType(starts->scalar_type(), false),
+                      "preference_loss: starts must hold 2 * pairs + 1 integers");
+    s->starts = on_device(*starts, s->rows.z, "starts").to(at::kLong).contiguous();
+    texts = starts->size(0) - 1;
+  } else {
+    texts = logit.size(0);
+    TORCH_CHECK_VALUE(logit.dim() >= 3 && texts % 2 == 0, "preference_loss: without starts, logit is [2 * pairs, rows, classes]");
+  }
+  s->P = to_int(texts / 2, "preference_loss");
+  if (ref_logp.has_value()) s->ref_logp = constant(*ref_logp, s->rows.z, texts, "ref_logp");
+  s->a = beta;
+  s->b = smoothing;
+  return choice_loss(logit, s);
+}
+
 void adam_step(const Tensor& w, const Tensor& g, const Tensor& m, const Tensor& v, double lr, double b1, double b2, double eps,
                double scale, const Tensor& steps) {
   const c10::cuda::CUDAGuard guard(w.device());
@@ -579,5 +836,9 @@ PYBIND11_MODULE(_native, m) {
   m.def("loss", &loss, py::call_guard<py::gil_scoped_release>());
   m.def("constraint_cost", &constraint_cost, py::call_guard<py::gil_scoped_release>());
   m.def("backward", &backward, py::call_guard<py::gil_scoped_release>());
+  m.def("embedding", &embedding, py::call_guard<py::gil_scoped_release>());
+  m.def("label_log_probs", &label_log_probs, py::call_guard<py::gil_scoped_release>());
+  m.def("policy_loss", &policy_loss, py::call_guard<py::gil_scoped_release>());
+  m.def("preference_loss", &preference_loss, py::call_guard<py::gil_scoped_release>());
   m.def("adam_step", &adam_step, py::call_guard<py::gil_scoped_release>());
 }

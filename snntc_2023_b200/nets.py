@@ -7,12 +7,13 @@ A network is described by a list of layer specs:
     ("pool", k)                      earliest-spike pooling, stride k, SAME
     ("flatten",)                     NHWC -> [B, H*W*C]
     ("dense", In, Out)
+    ("embed", tokens, D)             first layer of a network on tokens: ids [B,...] -> spike values [B,...,D]
 """
 import numpy as np
 import torch
 
 from . import _lib
-from .SNN_TC_Modules import SNN_conv, SNN_dense, SNN_maxpool2d, init_weight, loss_func
+from .SNN_TC_Modules import SNN_conv, SNN_dense, SNN_embedding, SNN_maxpool2d, init_weight, loss_func
 
 MNIST_MLP = [("dense", 784, 400), ("dense", 400, 400), ("dense", 400, 10)]
 CIFAR_CNN = [("conv", 3, 64, 3, 1), ("conv", 64, 64, 3, 1), ("pool", 2),
@@ -36,6 +37,9 @@ def spec_weights(specs, seed, biasvolt=1.0):
             fan_in, fan_out = s[3] * s[3] * s[1], s[2]
         elif s[0] == "dense":
             fan_in, fan_out = s[1], s[2]
+        elif s[0] == "embed":
+            out.append(rng.rand(s[1], s[2]).astype(np.float32))   # spike times in [0, 1), as of encoded pixels
+            continue
         else:
             continue
         w = rng.randn(fan_in, fan_out) * np.sqrt(15.0 / fan_in)
@@ -46,7 +50,8 @@ def spec_weights(specs, seed, biasvolt=1.0):
 
 
 def layer_work(specs, in_shape):
-    """Per weighted layer (R, I incl. bias row, J) for a batch of ONE sample of shape in_shape (H,W,C) or (N,)."""
+    """Per weighted layer (R, I incl. bias row, J) for a batch of ONE sample of shape in_shape (H,W,C) or (N,); for a network
+    on tokens the shape of one sample's ids."""
     import math
     shape = tuple(in_shape)
     rows = []
@@ -62,6 +67,8 @@ def layer_work(specs, in_shape):
             shape = (math.ceil(H / s[1]), math.ceil(W / s[1]), C)
         elif s[0] == "flatten":
             shape = (int(np.prod(shape)),)
+        elif s[0] == "embed":       # no sums over inputs: no work of this kind, but the next layer needs its dX
+            shape = shape + (s[2],); first = False
         elif s[0] == "dense":
             rows.append(dict(kind="dense", R=1, I=s[1] + 1, J=s[2], needs_dx=not first))
             shape = (s[2],); first = False
@@ -96,6 +103,9 @@ class SnnNet(torch.nn.Module):
                 layers.append(SNN_maxpool2d(s[1], s[1], "SAME"))
             elif s[0] == "flatten":
                 layers.append(torch.nn.Flatten())
+            elif s[0] == "embed":
+                w = None if weights is None else weights[wi]
+                layers.append(SNN_embedding(s[1], s[2], weight=w)); wi += 1
             else:
                 raise ValueError("unknown layer spec %r" % (s,))
         self.layers = torch.nn.ModuleList(layers)
@@ -105,19 +115,26 @@ class SnnNet(torch.nn.Module):
     def weighted_layers(self):
         return [l for l in self.layers if isinstance(l, (SNN_conv, SNN_dense))]
 
+    def parameter_layers(self):
+        """The layers whose weights lie in flat_param: the weighted ones, which sum inputs, and embeddings, which do not (no part
+        of the constraint cost)."""
+        return [l for l in self.layers if isinstance(l, (SNN_conv, SNN_dense, SNN_embedding))]
+
     def _flatten_storage(self):
-        ws = self.weighted_layers()
-        total = sum(l.weight.numel() for l in ws)
+        ws = self.parameter_layers()
+        # behind a table, whose size may be odd, the next weights start on 16 bytes again (the gap stays zero)
+        sizes = [-(-l.weight.numel() // 4) * 4 if isinstance(l, SNN_embedding) else l.weight.numel() for l in ws]
+        total = sum(sizes)
         dev = ws[0].weight.device
-        self.flat_param = torch.empty(total, dtype=torch.float32, device=dev)
+        self.flat_param = torch.zeros(total, dtype=torch.float32, device=dev)
         self.flat_grad = torch.zeros(total, dtype=torch.float32, device=dev)
         off = 0
-        for l in ws:
+        for l, size in zip(ws, sizes):
             n = l.weight.numel()
             self.flat_param[off:off + n].copy_(l.weight.data.reshape(-1))
             l.weight.data = self.flat_param[off:off + n].view_as(l.weight)
             l.grad_sink = self.flat_grad[off:off + n].view_as(l.weight)
-            off += n
+            off += size
 
     def forward(self, x):
         for l in self.layers:
@@ -137,7 +154,7 @@ class SnnNet(torch.nn.Module):
         """objective.backward(), after which flat_grad holds d objective / d weights: the operators' dW (written
         by the kernels) plus whatever autograd accumulated in a weight's .grad for the other terms. The .grad
         of every weight is left pointing at its slice of flat_grad, for optimisers that read .grad."""
-        ws = self.weighted_layers()
+        ws = self.parameter_layers()
         weights, sinks = [l.weight for l in ws], [l.grad_sink for l in ws]
         for w in weights:
             w.grad = None

@@ -358,3 +358,14 @@ def snn_minpool(X, Kh, Kw, Sh, Sw, padding="SAME", padvalue=1e5):
         pt = pl = 0
         Nh, Nw = (H - Kh) // Sh + 1, (W - Kw) // Sw + 1
     return _lib.native().minpool(X, Kh, Kw, Sh, Sw, pt, pl, Nh, Nw, float(padvalue))
+
+
+# ------------------------------------------------------------------------------------------ embedding
+def snn_embedding(ids, weight, scale=1.0, padding_idx=None, spikes=False, no_spike=1e5, grad_sink=None):
+    """Rows of `weight` [tokens, D] for integer ids (int32 or int64, any shape): [..., D] of scale * row or, with spikes=True,
+    exp(scale * row) -- rows of spike times encoded as train.encode(p, scale, one_minus=False) encodes pixels. Where an id
+    is `padding_idx` or outside the table, all D values are `no_spike` and nothing gets a gradient. Differentiable in
+    `weight`: every row's gradient is summed over its tokens in their order, the same bits every run. `grad_sink`: a tensor
+    that receives the gradient instead of autograd (written, not accumulated), as for the layers."""
+    return _lib.native().embedding(_tensor(ids, "ids"), _tensor(weight, "weight"), float(scale), bool(spikes), padding_idx,
+                                   float(no_spike), grad_sink)

@@ -1,0 +1,506 @@
+"""GPU tests of the losses on choices -- label log-probabilities, clipped policy loss, preference loss -- against float64
+evaluations of their formulas.
+
+Tolerances, with u = 2^-24 (half a step of float32), d_j = -z_j - max(-z): a term exp(d_j) of a row's sum is off by the rounding of
+d_j and of its product with log2(e), 2 |d_j| u, and by the exponential's own 2^-22 = 4 u at most; the sum of a row by its longest chain of
+additions, 64 u for the row lengths here (a lane adds at most 32 and the tree over lanes has 10 levels), which weights the terms'
+errors by p_j. So total is off by REL = (4 + 64 + 2 sum_j p_j |d_j|) u relative, lp by REL + |lp| u (its own rounding),
+p_j by REL + (2 |d_j| + 4 + 2) u relative, and a gradient factor * (p - onehot) by |factor| (p_j * that + 2 u) where factor is exact."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def _logits(R, J, seed, ignore=0.1):
+    """Spike values, three in ten without a spike, the first row without any; labels among the likelier half."""
+    import torch
+    g = torch.Generator("cuda").manual_seed(seed)
+    z = torch.rand(R, J, device="cuda", generator=g) * 6 + 1
+    z[torch.rand(R, J, device="cuda", generator=g) < 0.3] = 1e5
+    z[0] = 1e5
+    lab = (z + torch.rand(R, J, device="cuda", generator=g)).argmin(1)
+    lab[torch.rand(R, device="cuda", generator=g) < ignore] = -1
+    return z, lab
+
+
+class Ref:
+    """Softmax of the rows in float64 and the bounds of the module's docstring."""
+
+    def __init__(self, z, lab):
+        import torch
+        R, J = z.shape
+        self.counts = (lab >= 0) & (lab < J)
+        at = lab.clamp(0, J - 1)
+        x = -z.double()
+        x = torch.where(self.counts[:, None], x, torch.zeros_like(x))
+        self.lp = torch.where(self.counts, torch.log_softmax(x, 1).gather(1, at[:, None])[:, 0], 0.0)
+        self.p = torch.softmax(x, 1)
+        d = (x.amax(1, keepdim=True) - x).clamp(max=200.0)          # (beyond that p is 0 on both sides)
+        self.rel = (68 + 2 * (self.p * d).sum(1)) * U
+        self.p_rel = self.rel[:, None] + (2 * d + 6) * U
+        self.hot = torch.zeros_like(self.p)
+        self.hot[torch.arange(R, device=z.device), at] = 1.0
+
+    def check_lp(self, lp):
+        assert ((lp.double() - self.lp).abs() <= self.counts * (self.rel + self.lp.abs() * U) * 1.001).all()
+
+    def check_grad(self, grad, factor, factor_tol):
+        """factor: float64 per row; factor_tol: how far the kernel's may be off"""
+        import torch
+        factor, factor_tol = torch.where(self.counts, factor, 0.0)[:, None], torch.where(self.counts, factor_tol, 0.0)[:, None]
+        want = factor * (self.p - self.hot)
+        tol = factor.abs() * (self.p * self.p_rel + 2 * U * (self.p + self.hot)) + factor_tol * (self.p + self.hot) * 1.01 + 1e-38
+        err = (grad.double() - want).abs()
+        assert (err <= tol * 1.001).all(), float((err / tol).max())
+        assert (grad[~self.counts] == 0).all()
+
+
+SHAPES = [(1, 1), (1, 2), (3, 1), (2, 3), (37, 10), (257, 10), (5, 13), (6, 14), (7, 29), (4, 31), (5, 61), (65, 64), (9, 125), (3, 128), (8, 253),
+          (33, 257), (3, 509), (4, 1000), (130, 1000), (3, 1021), (2, 1024), (3, 2049), (5, 4093), (2, 8191), (3, 8192), (1, 8193), (2, 16381),
+          (2, 16385), (3, 32768), (2, 50021), (1, 65536), (2, 131070), (1, 131073), (1, 262147), (5000, 17), (40000, 2)]
+
+
+@pytest.mark.parametrize("R,J", SHAPES)
+def test_label_log_probs_and_their_gradient(R, J):
+    import torch
+    from snntc_2023_b200 import train
+    z, lab = _logits(R, J, R * 7 + J)
+    ref = Ref(z, lab)
+    z1 = z.clone().requires_grad_(True)
+    lp = train.label_log_probs(z1, lab)
+    assert lp.shape == (R,) and lp.dtype == torch.float32
+    ref.check_lp(lp.detach())
+    up = torch.randn(R, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    lp.backward(up)
+    ref.check_grad(z1.grad, up.double(), torch.zeros(R, dtype=torch.float64, device="cuda"))
+    with torch.no_grad():
+        assert torch.equal(train.label_log_probs(z1, lab), lp)
+    assert torch.equal(train.label_log_probs(z, lab.int()), lp.detach())
+
+
+def _policy_ref(ref, old, adv, refp, lo, hi, kl_coef):
+    """loss, stats and factors in float64; and how far an error of lp, ref.rel + u |lp| at most (the kernel keeps lp in 64 bits), moves
+    them. Rows whose ratio is nearer to the border than that are reported."""
+    import torch
+    n = max(1, int(ref.counts.sum()))
+    dlp = ref.rel
+    ratio = torch.exp(ref.lp - old.double())
+    a = adv.double()
+    near = torch.minimum((ratio - (1 + hi)).abs(), (ratio - (1 - lo)).abs()) <= ratio * dlp * 1.01 + 1e-12
+    clipped = ((a > 0) & (ratio > 1 + hi)) | ((a < 0) & (ratio < 1 - lo))
+    gain = torch.where(clipped, ratio.clamp(1 - lo, 1 + hi), ratio) * a
+    slope = torch.where(clipped, 0.0, -ratio * a)
+    slack = torch.where(clipped, 0.0, (ratio * a).abs() * dlp)
+    loss, kl = -gain, torch.zeros_like(a)
+    loss_slack, kl_slack = slack.clone(), torch.zeros_like(a)
+    if refp is not None:
+        away = refp.double() - ref.lp
+        kl = torch.expm1(away) - away
+        loss = loss + kl_coef * kl
+        slope = slope - kl_coef * torch.expm1(away)
+        slack = slack + abs(kl_coef) * torch.exp(away) * dlp
+        kl_slack = torch.expm1(away).abs() * dlp + torch.exp(away) * dlp ** 2
+        loss_slack = loss_slack + abs(kl_coef) * kl_slack
+    c = ref.counts
+    mean = lambda v: float(torch.where(c, v.double(), 0.0).sum()) / n  # noqa: E731
+    tiny = 1e-9        # the 64-bit arithmetic of a row, relative to its terms
+    sizes = gain.abs() + kl.abs() * abs(kl_coef)
+    return dict(loss=mean(loss), loss_tol=mean(loss_slack) * 1.01 + tiny * mean(sizes), kl=mean(kl), kl_tol=mean(kl_slack) * 1.01 + tiny * mean(kl.abs()),
+                clipped=mean(clipped), factor=slope / n, factor_tol=(slack * 1.01 + slope.abs() * (U + tiny)) / n, near=bool((near & c).any()))
+
+
+@pytest.mark.parametrize("R,J", SHAPES)
+@pytest.mark.parametrize("with_ref", [True, False])
+def test_policy_loss_and_its_gradient(R, J, with_ref):
+    import torch
+    from snntc_2023_b200 import train
+    z, lab = _logits(R, J, R + 3 * J)
+    ref = Ref(z, lab)
+    g = torch.Generator("cuda").manual_seed(4)
+    noise = lambda s: s * torch.randn(R, device="cuda", generator=g)  # noqa: E731
+    old, refp, adv = (ref.lp + noise(0.3)).float(), (ref.lp + noise(0.5)).float(), noise(1.0)
+    for t in (old, refp, adv):
+        t[~ref.counts] = float("nan")                 # what stands beside a row that does not count is not read
+    refp = refp if with_ref else None
+    kl_coef = 0.3 if with_ref else 0.0
+    want = _policy_ref(ref, old, adv, refp, 0.2, 0.25, kl_coef)
+    assert not want["near"], "a ratio lies on the border of the clip: another seed"
+    z1 = z.clone().requires_grad_(True)
+    loss, stats = train.policy_loss(z1, lab, old, adv, ref_logp=refp, clip_low=0.2, clip_high=0.25, kl_coef=kl_coef, with_stats=True)
+    assert loss.dim() == 0 and stats.shape == (2,) and not stats.requires_grad
+    close = lambda got, w, tol: abs(float(got) - w) <= tol + abs(w) * U + 1e-30  # noqa: E731
+    assert close(loss, want["loss"], want["loss_tol"]) and close(stats[0], want["kl"], want["kl_tol"]) and close(stats[1], want["clipped"], 1e-12)
+    loss.backward()
+    ref.check_grad(z1.grad, want["factor"], want["factor_tol"])
+    first = z1.grad.clone()
+    # an upstream factor other than one, twice over the same graph (the second time on top of the first)
+    z1.grad = None
+    again = train.policy_loss(z1, lab, old, adv, ref_logp=refp, clip_low=0.2, clip_high=0.25, kl_coef=kl_coef)
+    assert torch.equal(again, loss)
+    (again * -2.0).backward(retain_graph=True)
+    assert torch.equal(z1.grad, -2.0 * first)         # (a power of two moves no rounding)
+    again.backward()
+    assert torch.allclose(z1.grad, -first, rtol=1e-6, atol=1e-30)
+    with torch.no_grad():
+        alone = train.policy_loss(z1, lab, old, adv, ref_logp=refp, clip_low=0.2, clip_high=0.25, kl_coef=kl_coef, with_stats=True)
+    assert torch.equal(alone[0], loss) and torch.equal(alone[1], stats)
+
+
+def _texts(R, P, seed, tail):
+    """2P+1 ascending offsets, an empty text among them where there are several, `tail` rows behind the last."""
+    import random
+
+    import torch
+    rng = random.Random(seed)
+    cuts = sorted(rng.randrange(R - tail + 1) for _ in range(2 * P - 1))
+    if P > 1:
+        cuts[1] = cuts[0]
+    return torch.tensor([0] + cuts + [R - tail], device="cuda")
+
+
+def _preference_ref(ref, starts, refp, beta, eps):
+    import torch
+    b = starts.tolist()
+    P = (len(b) - 1) // 2
+    text = lambda v: torch.stack([v[x:y].sum() for x, y in zip(b[:-1], b[1:])])  # noqa: E731
+    s = text(ref.lp)
+    slack = text(torch.where(ref.counts, ref.rel, 0.0))
+    if refp is not None:
+        s = s - refp.double()
+    m = beta * (s[:P] - s[P:])
+    dm = abs(beta) * (slack[:P] + slack[P:]) * 1.01 + 1e-12 * (1 + s[:P].abs() + s[P:].abs())
+    sig = torch.sigmoid(m)
+    loss = -((1 - eps) * torch.nn.functional.logsigmoid(m) + eps * torch.nn.functional.logsigmoid(-m))
+    per = beta / P * (sig - (1 - eps))
+    per_tol = abs(beta) / P * dm / 4 + per.abs() * U * 1.01 + abs(beta) / P * 1e-15
+    factor, tol = torch.zeros_like(ref.lp), torch.zeros_like(ref.lp)
+    for k in range(P):
+        for t, sign in ((k, 1.0), (P + k, -1.0)):
+            factor[b[t]:b[t + 1]], tol[b[t]:b[t + 1]] = sign * per[k], per_tol[k]
+    return dict(loss=float(loss.mean()), loss_tol=float(dm.mean()), m=m, dm=dm, factor=factor, factor_tol=tol)
+
+
+@pytest.mark.parametrize("R,J,P,tail", [(2, 3, 1, 0), (7, 10, 1, 2), (37, 10, 5, 3), (64, 1000, 8, 0), (517, 333, 8, 20), (40, 8192, 3, 1), (24, 16390, 2, 4),
+                                        (12, 50021, 2, 1), (6, 131073, 1, 1), (3000, 5, 700, 100), (20000, 7, 1, 0), (10, 4, 30, 0)])
+@pytest.mark.parametrize("with_ref", [True, False])
+def test_preference_loss_and_its_gradient(R, J, P, tail, with_ref):
+    import torch
+    from snntc_2023_b200 import train
+    z, lab = _logits(R, J, R + J + P, ignore=0.2)
+    z[R - tail:] = float("nan")                       # rows behind the last text: no part in anything
+    lab[R - tail:] = -1
+    starts = _texts(R, P, R + P, tail)
+    ref = Ref(z, lab)
+    g = torch.Generator("cuda").manual_seed(6)
+    b = starts.tolist()
+    sums = torch.stack([ref.lp[x:y].sum() for x, y in zip(b[:-1], b[1:])])
+    refp = (sums + 4 * torch.randn(2 * P, device="cuda", generator=g)).float() if with_ref else None
+    beta, eps = (0.3, 0.1) if with_ref else (0.01, 0.0)
+    want = _preference_ref(ref, starts, refp, beta, eps)
+    z1 = z.clone().requires_grad_(True)
+    loss, m = train.preference_loss(z1, lab, starts, ref_logp=refp, beta=beta, label_smoothing=eps, with_margins=True)
+    assert m.shape == (P,) and not m.requires_grad
+    assert ((m.double() - want["m"]).abs() <= want["dm"] + want["m"].abs() * U).all()
+    assert abs(float(loss) - want["loss"]) <= want["loss_tol"] + abs(want["loss"]) * U
+    loss.backward()
+    ref.check_grad(z1.grad, want["factor"], want["factor_tol"])
+    first = z1.grad.clone()
+    z1.grad = None
+    again = train.preference_loss(z1, lab, starts.int(), ref_logp=refp, beta=beta, label_smoothing=eps)
+    (again * 4.0).backward()
+    assert torch.equal(again, loss) and torch.equal(z1.grad, 4.0 * first)
+    with torch.no_grad():
+        assert torch.equal(train.preference_loss(z1, lab, starts, ref_logp=refp, beta=beta, label_smoothing=eps), loss)
+
+
+def test_rows_of_a_text_that_a_label_leaves_out_but_no_text_owns():
+    """Rows behind the last text whose labels are classes: no gradient, whatever their logits."""
+    import torch
+    from snntc_2023_b200 import train
+    z, lab = _logits(20, 9, 2, ignore=0.0)
+    starts = torch.tensor([0, 6, 14], device="cuda")
+    z1 = z.clone().requires_grad_(True)
+    loss = train.preference_loss(z1, lab, starts, beta=0.01)
+    loss.backward()
+    assert (z1.grad[14:] == 0).all() and z1.grad[:14].abs().sum(1).gt(0).all()
+    short = train.preference_loss(z[:14], lab[:14], starts, beta=0.01)
+    assert torch.equal(short, loss.detach())
+
+
+def test_padded_texts_are_the_packed_ones():
+    import torch
+    from snntc_2023_b200 import train
+    z, lab = _logits(6 * 11, 50, 9, ignore=0.3)
+    zp, labp = z.view(6, 11, 50).clone().requires_grad_(True), lab.view(6, 11)
+    refp = torch.randn(6, device="cuda")
+    loss, m = train.preference_loss(zp, labp, ref_logp=refp, beta=0.2, with_margins=True)
+    loss.backward()
+    zq = z.clone().requires_grad_(True)
+    packed, mq = train.preference_loss(zq, lab, torch.arange(0, 67, 11, device="cuda"), ref_logp=refp, beta=0.2, with_margins=True)
+    packed.backward()
+    assert torch.equal(loss, packed) and torch.equal(m, mq) and torch.equal(zp.grad.view(66, 50), zq.grad)
+    lp = train.label_log_probs(zp, labp)
+    assert lp.shape == (6, 11) and torch.equal(lp.view(-1), train.label_log_probs(zq, lab))
+
+
+def test_offsets_that_are_no_offsets_stay_inside():
+    """Offsets that descend or leave the rows are held to them: numbers without meaning, but no access outside."""
+    import torch
+    from snntc_2023_b200 import train
+    z, lab = _logits(30, 12, 3)
+    for bad in ([5, 2, 28], [-7, 12, 10 ** 12], [0, 50, 40, 31, 60], [2 ** 62, -2 ** 62, 3]):
+        z1 = z.clone().requires_grad_(True)
+        loss = train.preference_loss(z1, lab, torch.tensor(bad, device="cuda"), beta=0.01)
+        loss.backward()
+        assert math.isfinite(float(loss.detach())) and z1.grad.isfinite().all()
+
+
+def test_no_row_counts():
+    import torch
+    from snntc_2023_b200 import train
+    for R, J in ((1, 5), (70, 10), (9, 2000), (3, 40000)):
+        z = torch.full((R, J), float("nan"), device="cuda", requires_grad=True)
+        lab = torch.full((R,), -1, device="cuda")
+        lab[0] = J
+        nan = torch.full((R,), float("nan"), device="cuda")
+        loss, stats = train.policy_loss(z, lab, nan, nan, ref_logp=nan, kl_coef=1.0, with_stats=True)
+        loss.backward()
+        assert float(loss) == 0 and (stats == 0).all() and (z.grad == 0).all()
+        z.grad = None
+        lp = train.label_log_probs(z, lab)
+        lp.sum().backward()
+        assert (lp == 0).all() and (z.grad == 0).all()
+        z.grad = None
+        loss = train.preference_loss(z, lab, torch.tensor([0, R, R], device="cuda"))
+        loss.backward()
+        assert abs(float(loss) - math.log(2)) < 1e-6 and (z.grad == 0).all()
+
+
+def test_infinite_and_nan_outputs():
+    """Outputs at +inf have no part in a softmax; a row with a NaN is NaN and touches no other row."""
+    import torch
+    from snntc_2023_b200 import train
+    for J in (7, 100, 700, 5000, 20000):
+        z, lab = _logits(6, J, J, ignore=0.0)
+        z[1:, 0] = float("inf")
+        lab[lab == 0] = 1
+        z[3, 2] = float("nan")
+        z1 = z.clone().requires_grad_(True)
+        lp = train.label_log_probs(z1, lab)
+        lp.sum().backward()
+        keep = [0, 1, 2, 4, 5]
+        zf = z[keep].clone()
+        zf[zf == float("inf")] = 1e30
+        ref = Ref(zf, lab[keep])
+        ref.check_lp(lp.detach()[keep])
+        ref.check_grad(z1.grad[keep], torch.ones(5, dtype=torch.float64, device="cuda"), torch.zeros(5, dtype=torch.float64, device="cuda"))
+        assert lp[3].isnan() and z1.grad[3, 1].isnan()
+
+
+def test_gradients_against_differences():
+    """Central differences of the losses in float64 (their formulas' own, at the kernels' inputs) along random directions: with steps of
+    1e-6 they are good to 1e-7 of the slope's size."""
+    import torch
+    from snntc_2023_b200 import train
+    g = torch.Generator("cuda").manual_seed(0)
+    R, J = 24, 40
+    z = torch.rand(R, J, device="cuda", generator=g) * 4 + 1
+    lab = torch.randint(0, J, (R,), device="cuda", generator=g)
+    lab[5] = -1
+    c = lab >= 0
+    lp_of = lambda y: torch.where(c, torch.log_softmax(-y, 1).gather(1, lab.clamp(min=0)[:, None])[:, 0], 0.0)  # noqa: E731
+    lp0 = lp_of(z.double())
+    old, refp, adv = (lp0 + 0.3 * torch.randn(R, device="cuda", generator=g)).float(), (lp0 - 0.2).float(), torch.randn(R, device="cuda", generator=g)
+    starts = torch.tensor([0, 6, 9, 9, 22], device="cuda")
+
+    def policy(y):
+        lp = lp_of(y)[c]
+        r, a, w = torch.exp(lp - old.double()[c]), adv.double()[c], refp.double()[c] - lp
+        return (0.4 * (torch.exp(w) - w - 1) - torch.minimum(r * a, r.clamp(0.8, 1.2) * a)).mean()
+
+    def preference(y):
+        s = torch.stack([lp_of(y)[i:j].sum() for i, j in ((0, 6), (6, 9), (9, 9), (9, 22))])
+        m = 0.2 * (s[:2] - s[2:])
+        return -(0.9 * torch.nn.functional.logsigmoid(m) + 0.1 * torch.nn.functional.logsigmoid(-m)).mean()
+
+    calls = ((policy, lambda y: train.policy_loss(y, lab, old, adv, ref_logp=refp, kl_coef=0.4)),
+             (preference, lambda y: train.preference_loss(y, lab, starts, beta=0.2, label_smoothing=0.1)),
+             (lambda y: lp_of(y).sum(), lambda y: train.label_log_probs(y, lab).sum()))
+    for plain, call in calls:
+        z1 = z.clone().requires_grad_(True)
+        (grad,) = torch.autograd.grad(call(z1), z1)
+        for _ in range(8):
+            v = torch.randn(R, J, device="cuda", dtype=torch.float64, generator=g)
+            slope = float((plain(z.double() + 1e-6 * v) - plain(z.double() - 1e-6 * v)) / 2e-6)
+            size = float((grad.double() * v).abs().sum())
+            assert abs(float((grad.double() * v).sum()) - slope) <= 2e-6 * size      # 1e-7 of the difference, the rest float32's p and factors
+
+
+def test_strides_offsets_and_leading_dimensions():
+    import torch
+    from snntc_2023_b200 import train
+    z, lab = _logits(60, 33, 11)
+    wide = torch.rand(60, 80, device="cuda")
+    wide[:, 7:40] = z
+    base = wide.clone().requires_grad_(True)
+    lp = train.label_log_probs(base[:, 7:40], lab)
+    lp.sum().backward()
+    z1 = z.clone().requires_grad_(True)
+    plain = train.label_log_probs(z1, lab)
+    plain.sum().backward()
+    assert torch.equal(lp, plain) and torch.equal(base.grad[:, 7:40], z1.grad) and not base.grad[:, :7].any() and not base.grad[:, 40:].any()
+    for off in (1, 2, 3):                             # contiguous rows that start off 16 bytes
+        for J in (33, 1028, 9000):
+            zz, ll = _logits(7, J, off + J)
+            buf = torch.empty(off + zz.numel(), device="cuda")
+            moved = buf[off:].view(7, J).copy_(zz).detach().requires_grad_(True)
+            zz.requires_grad_(True)
+            adv = torch.randn(7, device="cuda")
+            old = train.label_log_probs(zz, ll).detach() - 0.1
+            a, b = (train.policy_loss(t, ll, old, adv) for t in (moved, zz))
+            a.backward()
+            b.backward()
+            assert torch.allclose(a, b, rtol=1e-5) and torch.allclose(moved.grad, zz.grad, rtol=1e-5, atol=1e-9)
+    zl, ll = z.view(3, 4, 5, 33), lab.view(3, 4, 5)
+    assert torch.equal(train.label_log_probs(zl.transpose(0, 1), ll.transpose(0, 1)), plain.detach().view(3, 4, 5).transpose(0, 1))
+
+
+def test_more_than_32_bits_of_logits():
+    import torch
+    from snntc_2023_b200 import train
+    R, J = 66000, 32800                               # 2.16e9 logits
+    z = torch.full((R, J), 4.0, device="cuda")
+    z[:, 5] = 1.0
+    z[-1, J - 1] = 0.5
+    lab = torch.full((R,), -1, device="cuda")
+    lab[0], lab[R // 2], lab[R - 1] = 5, 5, J - 1
+    z.requires_grad_(True)
+    lp = train.label_log_probs(z, lab)
+    rows = torch.tensor([0, R // 2, R - 1], device="cuda")
+    ref = Ref(z.detach()[rows], lab[rows])
+    ref.check_lp(lp.detach()[rows])
+    old = lp.detach() - 0.05
+    del lp
+    loss = train.policy_loss(z, lab, old, torch.ones(R, device="cuda"))
+    (grad,) = torch.autograd.grad(loss, z)
+    f = -torch.exp(ref.lp - old[rows].double()) / 3
+    ref.check_grad(grad[rows], f, f.abs() * (ref.rel * 1.1 + 2 * U))
+    grad[rows] = 0
+    assert not grad.any()
+
+
+def test_refusals():
+    import torch
+    from snntc_2023_b200 import _lib, train
+    z, lab = _logits(8, 5, 1)
+    v = torch.zeros(8, device="cuda")
+    for bad in (z.double(), z.half(), z[0], z[:0], z[:, :0], z.view(2, 4, 5)):
+        with pytest.raises(ValueError):
+            train.label_log_probs(bad, lab[:bad.shape[0]] if bad.dim() == 2 and bad.shape[0] == 0 else lab)
+    for bad in (lab.float(), lab.bool(), lab[:7], lab.view(2, 4)):
+        with pytest.raises(ValueError):
+            train.label_log_probs(z, bad)
+    with pytest.raises(ValueError):
+        train.policy_loss(z, lab, v[:7], v)
+    with pytest.raises(ValueError):
+        train.policy_loss(z, lab, v, v.double())
+    with pytest.raises(_lib.SnntcError):
+        train.policy_loss(z, lab, v.cpu(), v)
+    with pytest.raises(ValueError, match="detach"):
+        train.policy_loss(z, lab, v, v.clone().requires_grad_(True))
+    with pytest.raises(ValueError, match="ref_logp"):
+        train.policy_loss(z, lab, v, v, kl_coef=0.1)
+    for kw in (dict(clip_low=-0.1), dict(clip_low=1.5), dict(clip_high=-1.0), dict(clip_high=float("nan")), dict(kl_coef=float("inf"), ref_logp=v)):
+        with pytest.raises(ValueError):
+            train.policy_loss(z, lab, v, v, **kw)
+    starts = torch.tensor([0, 4, 8], device="cuda")
+    for bad in (None, starts[:2], starts[:1], starts.float(), starts.view(1, 3), starts.cpu()):
+        with pytest.raises(ValueError):
+            train.preference_loss(z, lab, bad)
+    for kw in (dict(beta=float("nan")), dict(label_smoothing=-0.1), dict(label_smoothing=2.0), dict(ref_logp=v)):
+        with pytest.raises(ValueError):
+            train.preference_loss(z, lab, starts, **kw)
+    with pytest.raises(ValueError):
+        train.preference_loss(z.view(1, 8, 5), lab.view(1, 8))            # an odd number of padded texts
+    z1 = z.clone().requires_grad_(True)
+    for loss in (train.label_log_probs(z1, lab).sum(), train.policy_loss(z1, lab, v, v), train.preference_loss(z1, lab, starts)):
+        with pytest.raises(RuntimeError, match="create_graph"):
+            torch.autograd.grad(loss, z1, create_graph=True)
+    loss = train.policy_loss(z1, lab, v, v)
+    with torch.no_grad():
+        z1 += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def _all_losses(z, lab, old, adv, refp, starts):
+    import torch
+    from snntc_2023_b200 import train
+    out = []
+    for loss in (train.policy_loss(z, lab, old, adv, ref_logp=refp, kl_coef=0.1), train.preference_loss(z, lab, starts, beta=0.05),
+                 (train.label_log_probs(z, lab) * adv).sum()):
+        out += [loss.detach(), torch.autograd.grad(loss, z)[0]]
+    return out
+
+
+@pytest.mark.parametrize("R,J", [(64, 10), (300, 500), (40, 20011)])
+def test_captured_replayed_and_on_other_streams(R, J):
+    """Forward and gradient captured once and replayed on other inputs; two captured graphs and plain calls on two streams at once."""
+    import torch
+    sets = []
+    for k in range(2):
+        z, lab = _logits(R, J, 50 + k)
+        sets.append((z, lab, -2 - torch.rand(R, device="cuda"), torch.randn(R, device="cuda"), -2 - torch.rand(R, device="cuda"),
+                     torch.tensor([0, R // 4 + k, R // 2, R // 2, R - k], device="cuda")))
+    plain = [_all_losses(s[0].clone().requires_grad_(True), *s[1:]) for s in sets]
+    graphs = []
+    for k in range(2):
+        own = [t.clone() for t in sets[k]]
+        own[0].requires_grad_(True)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            _all_losses(*own)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = _all_losses(*own)
+        graphs.append((graph, own, out))
+    same = lambda a, b: all(torch.equal(x, y) for x, y in zip(a, b))  # noqa: E731
+    graph, own, out = graphs[0]
+    for k in (1, 0):
+        with torch.no_grad():
+            for dst, src in zip(own, sets[k]):
+                dst.copy_(src)
+        graph.replay()
+        assert same(out, plain[k])
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                graphs[k][0].replay()
+            with torch.cuda.stream(streams[2 + k]):
+                got[k].append(_all_losses(sets[k][0].clone().requires_grad_(True), *sets[k][1:]))
+    torch.cuda.synchronize()
+    assert all(same(g, plain[k]) for k in range(2) for g in got[k])
+    assert same(graphs[0][2], plain[0]) and same(graphs[1][2], plain[1])
+
+
+def test_a_capture_beside_a_live_eager_graph_is_refused():
+    import torch
+    from snntc_2023_b200 import train
+    z, lab = _logits(16, 9, 1)
+    z.requires_grad_(True)
+    alive = train.label_log_probs(z, lab)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            train.label_log_probs(z, lab).sum().backward()
+    torch.cuda.synchronize()
+    alive.sum().backward()
+    assert z.grad.isfinite().all()

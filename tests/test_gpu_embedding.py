@@ -1,0 +1,232 @@
+"""GPU tests of the embedding and its gradient against float64 evaluations of their formulas.
+
+Tolerances, with u = 2^-24 (half a step of float32): scale * e is one rounding, u relative. exp(scale * e): the argument's
+rounding, |scale e| u, and expf's two units in the last place, 4 u, so (|scale e| + 5) u. A sum of n terms in any order is off by
+at most n u times the sum of their magnitudes; with the factor (the above and one product) (n + |scale e| + 8) u."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def _case(N, V, D, seed, dtype=None, skew=False):
+    import torch
+    g = torch.Generator("cuda").manual_seed(seed)
+    ids = torch.randint(0, V, (N,), device="cuda", generator=g, dtype=dtype or torch.int64)
+    if skew:                                         # half of the tokens are one id
+        ids[torch.rand(N, device="cuda", generator=g) < 0.5] = V // 2
+    table = torch.rand(V, D, device="cuda", generator=g) * 2 - 0.5
+    up = torch.randn(N, D, device="cuda", generator=g)
+    return ids, table, up
+
+
+def _check(ids, table, up, y, grad, scale, spikes, padding=None, no_spike=1e5):
+    """y and grad against the formulas; ids outside the table allowed."""
+    import torch
+    V, D = table.shape
+    flat = ids.reshape(-1).long()
+    there = (flat >= 0) & (flat < V)
+    if padding is not None:
+        there &= flat != padding
+    at = flat.clamp(0, V - 1)
+    arg = table.double() * float(np.float32(scale))
+    value = arg.exp() if spikes else arg
+    want = torch.where(there[:, None], value[at], torch.full((), no_spike, dtype=torch.float64, device=y.device))
+    tol = want.abs() * U * ((arg[at].abs() + 5) if spikes else 1) * 1.0001
+    assert ((y.reshape(-1, D).double() - want).abs() <= torch.where(there[:, None], tol, torch.zeros_like(tol))).all()
+    if grad is None:
+        return
+    f = float(np.float32(scale)) * (value if spikes else torch.ones_like(value))
+    total = torch.zeros(V, D, dtype=torch.float64, device=y.device).index_put_((at[there],), up.reshape(-1, D)[there].double(), accumulate=True)
+    size = torch.zeros(V, D, dtype=torch.float64, device=y.device).index_put_((at[there],), up.reshape(-1, D)[there].double().abs(), accumulate=True)
+    n = torch.bincount(at[there], minlength=V)[:, None].double()
+    bound = (n + (arg.abs() if spikes else 0) + 8) * U * size * f.abs()
+    err = (grad.double() - total * f).abs()
+    assert (err <= bound).all(), float((err / bound.clamp(min=1e-300)).max())
+    assert (grad[n[:, 0] == 0] == 0).all()
+
+
+SIZES = [(1, 1, 1), (1, 10007, 784), (2, 2, 3), (31, 7, 4), (32, 1, 33), (33, 300, 128), (257, 255, 129), (257, 256, 64), (300, 257, 100),
+         (1000, 65536, 12), (4097, 1000, 100), (5000, 3, 257), (7007, 50021, 129), (20000, 65535, 36), (40000, 131072, 8), (70001, 90, 16),
+         (3, 100, 5000), (65536, 1 << 20, 4)]
+
+
+@pytest.mark.parametrize("N,V,D", SIZES)
+@pytest.mark.parametrize("spikes", [False, True])
+def test_values_and_gradient(N, V, D, spikes):
+    import torch
+    from snntc_2023_b200 import ops
+    ids, table, up = _case(N, V, D, N + V + D, skew=N % 2 == 1)
+    w = table.clone().requires_grad_(True)
+    y = ops.snn_embedding(ids, w, scale=1.5, spikes=spikes)
+    assert y.shape == (N, D)
+    y.backward(up)
+    _check(ids, table, up, y.detach(), w.grad, 1.5, spikes)
+    first = w.grad.clone()                           # the same bits again
+    w.grad = None
+    ops.snn_embedding(ids, w, scale=1.5, spikes=spikes).backward(up)
+    assert torch.equal(first, w.grad)
+    with torch.no_grad():
+        assert torch.equal(ops.snn_embedding(ids, w, scale=1.5, spikes=spikes), y)
+
+
+@pytest.mark.parametrize("bits", [32, 64])
+@pytest.mark.parametrize("N,V,D", [(129, 50, 24), (9000, 700, 33)])
+def test_padding_and_ids_outside_the_table_never_spike(bits, N, V, D):
+    import torch
+    from snntc_2023_b200 import ops
+    dtype = torch.int32 if bits == 32 else torch.int64
+    ids, table, up = _case(N, V, D, 5, dtype)
+    ids[::7] = -1
+    ids[1::11] = V
+    ids[2::13] = torch.iinfo(dtype).max if bits == 32 else 2 ** 40 + 3      # (the low 32 bits are an id of the table)
+    ids[5::17] = torch.iinfo(dtype).min
+    ids[3::5] = 4
+    up[::7] = float("nan")                           # what comes back for a token that does not spike is not read
+    w = table.clone().requires_grad_(True)
+    y = ops.snn_embedding(ids, w, scale=0.5, padding_idx=4, spikes=True, no_spike=2e5)
+    y.backward(up)
+    _check(ids, table, up, y.detach(), w.grad, 0.5, True, padding=4, no_spike=2e5)
+    assert (w.grad[4] == 0).all() and (y[::7] == 2e5).all()
+
+
+def test_no_token_at_all_and_no_ids():
+    import torch
+    from snntc_2023_b200 import ops
+    w = torch.rand(9, 4, device="cuda").requires_grad_(True)
+    y = ops.snn_embedding(torch.full((6,), -1, device="cuda"), w)
+    y.backward(torch.ones_like(y))
+    assert (y == 1e5).all() and (w.grad == 0).all()
+    w.grad = None
+    y = ops.snn_embedding(torch.empty(2, 0, dtype=torch.long, device="cuda"), w)
+    assert y.shape == (2, 0, 4)
+    y.sum().backward()
+    assert (w.grad == 0).all()
+
+
+def test_one_id_everywhere():
+    """A run over all tiles: every partial sum is of the same row."""
+    import torch
+    from snntc_2023_b200 import ops
+    for N, D in ((100000, 20), (5001, 512)):
+        ids, table, up = _case(N, 40, D, 8)
+        ids.fill_(39)
+        w = table.clone().requires_grad_(True)
+        y = ops.snn_embedding(ids, w, scale=2.0)
+        y.backward(up)
+        _check(ids, table, up, y.detach(), w.grad, 2.0, False)
+
+
+def test_strides_shapes_and_offsets():
+    import torch
+    from snntc_2023_b200 import ops
+    g = torch.Generator("cuda").manual_seed(2)
+    big = torch.rand(50, 14, device="cuda", generator=g)
+    ids = torch.randint(0, 50, (6, 8, 2), device="cuda", generator=g)
+    w = big[:, 1:14].requires_grad_(True)                                     # strided rows, off 16 bytes
+    y = ops.snn_embedding(ids.transpose(0, 1), w, spikes=True)
+    assert y.shape == (8, 6, 2, 13)
+    up = torch.randn(13, 8, 6, 2, device="cuda", generator=g).permute(1, 2, 3, 0)   # an upstream gradient with other strides
+    (grad,) = torch.autograd.grad(y, w, up)
+    _check(ids.transpose(0, 1).contiguous(), big[:, 1:14].contiguous(), up.contiguous(), y.detach(), grad, 1.0, True)
+    flat = torch.rand(1 + 30 * 8, device="cuda", generator=g)                 # a contiguous table that starts off 16 bytes
+    w = flat[1:].view(30, 8).detach().requires_grad_(True)
+    ids = torch.randint(0, 30, (777,), device="cuda", generator=g)
+    y = ops.snn_embedding(ids, w)
+    (grad,) = torch.autograd.grad(y.sum(), w)                                 # (the upstream gradient is one number, expanded)
+    _check(ids, w.detach(), torch.ones(777, 8, device="cuda"), y.detach(), grad, 1.0, False)
+
+
+def test_a_table_beyond_32_bit_offsets():
+    import torch
+    from snntc_2023_b200 import ops
+    V, D = 2_200_003, 1001                                                    # 2.2e9 elements
+    table = torch.empty(V, D, device="cuda")
+    ids = torch.tensor([0, V - 1, 2_150_000, V - 1, 7], device="cuda")
+    table[ids] = torch.rand(5, D, device="cuda")
+    w = table.requires_grad_(True)
+    y = ops.snn_embedding(ids, w, scale=3.0)
+    assert torch.equal(y.detach(), table.detach()[ids] * 3.0)
+    up = torch.randn(5, D, device="cuda")
+    (grad,) = torch.autograd.grad(y, w, up)
+    assert torch.equal(grad[V - 1], 3.0 * (up[1] + up[3])) and torch.equal(grad[2_150_000], 3.0 * up[2])
+    assert torch.equal(grad[0], 3.0 * up[0]) and torch.equal(grad[7], 3.0 * up[4])
+    grad[ids] = 0
+    assert not grad.any()
+
+
+def test_refusals():
+    import torch
+    from snntc_2023_b200 import ops
+    w = torch.rand(5, 4, device="cuda").requires_grad_(True)
+    ids = torch.zeros(3, dtype=torch.long, device="cuda")
+    for bad in (ids.float(), ids.bool(), ids.short(), ids.cpu()):
+        with pytest.raises(ValueError):
+            ops.snn_embedding(bad, w)
+    for bad in (w.double(), w.half(), w[0], w[:0]):
+        with pytest.raises(ValueError):
+            ops.snn_embedding(ids, bad)
+    with pytest.raises(ValueError):
+        ops.snn_embedding(ids, w, scale=float("nan"))
+    for sink in (torch.zeros(4, 5, device="cuda"), torch.zeros(5, 8, device="cuda")[:, ::2], torch.zeros(5, 4)):
+        with pytest.raises(ValueError):
+            ops.snn_embedding(ids, w, grad_sink=sink)
+    y = ops.snn_embedding(ids, w)
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(y.sum(), w, create_graph=True)
+
+
+def test_captured_replayed_and_on_another_stream():
+    """Lookup and gradient captured once, replayed on other ids; and two streams at once: the results of plain calls."""
+    import torch
+    from snntc_2023_b200 import ops
+    N, V, D = 3001, 500, 36
+    ids, table, up = _case(N, V, D, 1)
+    w = table.clone().requires_grad_(True)
+
+    def step(i, g):
+        y = ops.snn_embedding(i, w, spikes=True)
+        return y.detach(), torch.autograd.grad(y, w, g)[0]
+
+    other = (torch.randint(-1, V, (N,), device="cuda"), torch.randn(N, D, device="cuda"))
+    plain = [step(ids, up), step(*other)]
+    sid, sup = ids.clone(), up.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(sid, sup)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(sid, sup)
+    for k, (i, g) in enumerate(((ids, up), other, (ids, up))):
+        sid.copy_(i)
+        sup.copy_(g)
+        graph.replay()
+        assert torch.equal(out[0], plain[k % 2][0]) and torch.equal(out[1], plain[k % 2][1])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(10):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(step(*((ids, up), other)[k]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, plain[k][0]) and torch.equal(b, plain[k][1]) for k in range(2) for a, b in got[k])
+
+
+def test_a_capture_beside_a_live_eager_graph_is_refused():
+    """Autograd would run the leaf's accumulation on the eager graph's stream, inside the capture. The call says so instead."""
+    import torch
+    from snntc_2023_b200 import ops
+    ids, table, up = _case(64, 20, 8, 1)
+    w = table.clone().requires_grad_(True)
+    alive = ops.snn_embedding(ids, w)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            ops.snn_embedding(ids, w).backward(up)
+    torch.cuda.synchronize()
+    alive.backward(up)                               # the eager graph is as it was
+    _check(ids, table, up, alive.detach(), w.grad, 1.0, False)
