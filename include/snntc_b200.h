@@ -212,7 +212,9 @@ SNNTC_API int snntc_sgdm_step(float* w, const float* g, float* vel, size_t n, fl
  * snntc_policy_loss  the mean over the rows that count of -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * k with
  *                    r = exp(lp - old_logp), A = advantage, k = exp(ref_logp - lp) - (ref_logp - lp) - 1. *loss and
  *                    kl_and_clipped[2] (mean k; share of rows whose ratio was clipped) are written; 0 where no row counts.
- *                    ref_logp may be null where kl_coef is 0.
+ *                    ref_logp may be null where kl_coef is 0. dz[R,J], where it is not null, receives dloss / dz in the pass that
+ *                    reads z. stats_2R and factor may be null.
+ * snntc_scale_gradient      dz *= *gout, n elements; nothing is moved where *gout is 1.
  * snntc_preference_loss  texts 0..P-1 are preferred to texts P..2P-1: text s is rows [starts[s], starts[s+1]) (2P+1 ascending
  *                    offsets, device; they are held to [0, R]) or, where starts is null, the s-th of 2P equal parts of the rows.
  *                    margins[k] = beta * ((S_k - ref_k) - (S_{P+k} - ref_{P+k})) with S the sum of a text's log-probabilities
@@ -232,8 +234,9 @@ SNNTC_API int snntc_choice_backward(const float* z, const long long* labels, con
 SNNTC_API size_t snntc_policy_loss_workspace_bytes(long long R);
 SNNTC_API int snntc_policy_loss(const float* z, const long long* labels, const float* old_logp, const float* advantage,
                                 const float* ref_logp, float* loss, float* kl_and_clipped, float* stats_2R, float* factor,
-                                long long R, int J, double clip_low, double clip_high, double kl_coef, void* workspace,
+                                float* dz, long long R, int J, double clip_low, double clip_high, double kl_coef, void* workspace,
                                 size_t workspace_bytes, void* stream);
+SNNTC_API int snntc_scale_gradient(float* dz, const float* gout, size_t n, void* stream);
 SNNTC_API size_t snntc_preference_loss_workspace_bytes(long long R, int P);
 SNNTC_API int snntc_preference_loss(const float* z, const long long* labels, const long long* starts, const float* ref_logp,
                                     float* loss, float* margins, float* stats_2R, float* factor, long long R, int J, int P,

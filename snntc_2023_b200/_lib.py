@@ -54,7 +54,8 @@ SYMBOLS = {
     "snntc_label_logp_forward": (_INT, [_F] * 4 + [_LL, _INT, _F]),
     "snntc_choice_backward": (_INT, [_F] * 6 + [_LL, _INT, _F]),
     "snntc_policy_loss_workspace_bytes": (_SZ, [_LL]),
-    "snntc_policy_loss": (_INT, [_F] * 9 + [_LL, _INT] + [ctypes.c_double] * 3 + [_F, _SZ, _F]),
+    "snntc_scale_gradient": (_INT, [_F, _F, _SZ, _F]),
+    "snntc_policy_loss": (_INT, [_F] * 10 + [_LL, _INT] + [ctypes.c_double] * 3 + [_F, _SZ, _F]),
     "snntc_preference_loss_workspace_bytes": (_SZ, [_LL, _INT]),
     "snntc_preference_loss": (_INT, [_F] * 8 + [_LL, _INT, _INT] + [ctypes.c_double] * 2 + [_F, _SZ, _F]),
 }

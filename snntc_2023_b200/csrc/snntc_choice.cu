@@ -12,93 +12,36 @@
 #include "../../include/snntc_b200.h"
 #include "snntc_launch.cuh"
 
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <float.h>
+#include <math_constants.h>
 #include <stdint.h>
 
 namespace snntc { void count_launch(int n = 1); void note_cuda_error(cudaError_t e); }
 
 namespace {
 
+namespace cg = cooperative_groups;
 using snntc::chain_next;
 using snntc::chain_wait;
 using snntc::launch_chained;
 using snntc::ld_plain;
 
-constexpr int kRowThreads = 256;
-
-// (running maximum, sum of exp(x - maximum)) of the logits x that a lane has seen. The maximum starts at the lowest finite value,
-// not at -inf, whose difference from itself is no number.
-struct Online {
-  float top = -FLT_MAX, total = 0.f;
-  __device__ __forceinline__ void add(float x) {
-    const float t = fmaxf(top, x);
-    total = total * expf(top - t) + expf(x - t);
-    top = t;
-  }
-  __device__ __forceinline__ void join(float t2, float s2) {
-    const float t = fmaxf(top, t2);
-    total = total * expf(top - t) + s2 * expf(t2 - t);
-    top = t;
-  }
-};
-
 __device__ __forceinline__ bool counts(long long label, int J) { return label >= 0 && label < J; }
+
+// exp(d) for d <= 0 as 2^(d log2 e), one product and one instruction: off by 2^-22 + |d| 2^-23 relative. The terms of a row's sum
+// and its probabilities are all it is used for; what is one number per row takes exp and log in 64 bits.
+__device__ __forceinline__ float exp_term(float d) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * 1.44269504f));
+  return e;
+}
+
+constexpr int kSumThreads = 1024;
 
 __device__ __forceinline__ double label_logp(float z_label, float2 st) {
   return (-(double)z_label - (double)st.x) - log((double)st.y);
-}
-
-// One warp per row: (top, total) and lp
-__global__ void __launch_bounds__(kRowThreads)
-choice_rows_kernel(const float* z, const long long* labels, float* __restrict__ logp, double* __restrict__ logp64,
-                   float2* __restrict__ stats, float* __restrict__ factor, long long R, int J) {
-  chain_wait();
-  chain_next();
-  const long long r = ((long long)blockIdx.x * kRowThreads + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (r >= R) return;
-  const long long label = ld_plain(labels + r);
-  Online o;
-  double lp = 0.0;
-  if (counts(label, J)) {
-    const float* row = z + r * J;
-    for (int j = lane; j < J; j += 32) o.add(-ld_plain(row + j));
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) {
-      const float t = __shfl_xor_sync(0xffffffffu, o.top, d), s = __shfl_xor_sync(0xffffffffu, o.total, d);
-      o.join(t, s);
-    }
-    lp = label_logp(ld_plain(row + label), make_float2(o.top, o.total));
-  }
-  if (lane == 0) {
-    if (logp) logp[r] = (float)lp;
-    if (logp64) logp64[r] = lp;
-    if (stats) stats[r] = make_float2(o.top, o.total);
-    if (factor) factor[r] = 0.f;
-  }
-}
-
-// dz = factor * (p - onehot), one warp per row
-__global__ void __launch_bounds__(kRowThreads)
-choice_grad_kernel(const float* z, const long long* labels, const float2* stats, const float* factor, const float* gout,
-                   float* __restrict__ dz, long long R, int J) {
-  chain_wait();
-  chain_next();
-  const long long r = ((long long)blockIdx.x * kRowThreads + threadIdx.x) >> 5;
-  const int lane = threadIdx.x & 31;
-  if (r >= R) return;
-  const long long label = ld_plain(labels + r);
-  const float f = ld_plain(factor + r) * (gout ? ld_plain(gout) : 1.f);
-  const float* row = z + r * J;
-  float* to = dz + r * J;
-  if (!counts(label, J) || f == 0.f) {
-    for (int j = lane; j < J; j += 32) to[j] = 0.f;
-    return;
-  }
-  const float2 st = ld_plain(stats + r);
-  const float inv = 1.f / st.y;
-  for (int j = lane; j < J; j += 32) to[j] = f * (expf(-ld_plain(row + j) - st.x) * inv - (j == label ? 1.f : 0.f));
 }
 
 struct PolicyParams { double lower, upper, kl_coef; };
@@ -143,34 +86,302 @@ __device__ __forceinline__ double3 block_sum(double3 v) {
   return t;
 }
 
-// One CTA: the terms of all rows, the mean over those that count, and the factors of the gradient.
-__global__ void __launch_bounds__(1024)
-policy_rows_kernel(const double* lp, const long long* labels, const float* old, const float* adv, const float* ref,
-                   float* __restrict__ factor, float* __restrict__ loss, float* __restrict__ out2, long long R, int J,
-                   PolicyParams q) {
+// Sum of three numbers over a cluster in a fixed order, the same value in all threads
+__device__ __forceinline__ double3 cluster_sum(double3 v) {
+  __shared__ double3 mine;
+  cg::cluster_group cl = cg::this_cluster();
+  v = block_sum(v);
+  if (threadIdx.x == 0) mine = v;
+  cl.sync();
+  double3 t = make_double3(0, 0, 0);
+  for (unsigned k = 0; k < cl.num_blocks(); ++k) {
+    const double3 o = *cl.map_shared_rank(&mine, k);
+    t.x += o.x;
+    t.y += o.y;
+    t.z += o.z;
+  }
+  cl.sync();                                   // no CTA leaves, or comes back, while its number may still be read
+  return t;
+}
+
+// How many rows count. One cluster: 65 536 labels are eight loads a thread.
+__global__ void __launch_bounds__(kSumThreads)
+policy_count_kernel(const long long* labels, double* __restrict__ inv_n, long long R, int J) {
   chain_wait();
   chain_next();
-  __shared__ double inv_n;
   double3 n = make_double3(0, 0, 0);
-  for (long long r = threadIdx.x; r < R; r += blockDim.x) n.x += counts(ld_plain(labels + r), J) ? 1.0 : 0.0;
-  n = block_sum(n);
-  if (threadIdx.x == 0) inv_n = n.x > 0 ? 1.0 / n.x : 0.0;
-  __syncthreads();
+  for (long long r = (long long)blockIdx.x * kSumThreads + threadIdx.x; r < R; r += (long long)gridDim.x * kSumThreads)
+    n.x += counts(ld_plain(labels + r), J) ? 1.0 : 0.0;
+  n = cluster_sum(n);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *inv_n = n.x > 0 ? 1.0 / n.x : 0.0;
+}
+
+__global__ void __launch_bounds__(kSumThreads)
+policy_mean_kernel(const double3* terms, const double* inv_n, float* __restrict__ loss, float* __restrict__ out2, long long R) {
+  chain_wait();
+  chain_next();
   double3 sum = make_double3(0, 0, 0);
-  for (long long r = threadIdx.x; r < R; r += blockDim.x) {
-    if (!counts(ld_plain(labels + r), J)) continue;
-    const PolicyRow p = policy_row(ld_plain(lp + r), ld_plain(old + r), ld_plain(adv + r), ref != nullptr, ref ? ld_plain(ref + r) : 0.f, q);
-    sum.x += p.loss;
-    sum.y += p.kl;
-    sum.z += p.clipped ? 1.0 : 0.0;
-    factor[r] = (float)(p.slope * inv_n);
+  for (long long r = (long long)blockIdx.x * kSumThreads + threadIdx.x; r < R; r += (long long)gridDim.x * kSumThreads) {
+    const double3 t = ld_plain(terms + r);
+    sum.x += t.x;
+    sum.y += t.y;
+    sum.z += t.z;
   }
-  sum = block_sum(sum);
-  if (threadIdx.x == 0) {
-    *loss = (float)(sum.x * inv_n);
-    out2[0] = (float)(sum.y * inv_n);
-    out2[1] = (float)(sum.z * inv_n);
+  sum = cluster_sum(sum);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    const double inv = ld_plain(inv_n);
+    *loss = (float)(sum.x * inv);
+    out2[0] = (float)(sum.y * inv);
+    out2[1] = (float)(sum.z * inv);
   }
+}
+
+// ---- rows. A group of G lanes (part of a warp, a warp, a CTA, or the CTAs of a cluster) holds a row in registers, NV vectors of four
+// a lane, all loads in flight at once: the row is read from memory once, and where the loss's factor follows from the row alone
+// (the policy loss), its gradient is written in the same pass. Rows of any length start anywhere, so a row is seen through the
+// 16-byte vectors that cover it; those that stick out at its ends are loaded and stored by element.
+// Maxima are a warp's own: every warp sums exp(x - its maximum), and one exchange joins (maximum, sum) pairs.
+template <int NV>
+struct RowValues { float x[4 * NV]; };
+
+// x = -z of the vectors first, first + stride, ...; -inf outside the row
+template <int NV>
+__device__ __forceinline__ RowValues<NV> load_row(const float* row, int J, bool live, int first, int stride) {
+  RowValues<NV> v;
+  const int lead = (int)(((uintptr_t)row >> 2) & 3);
+  const float4* base = (const float4*)(row - lead);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int at = first + k * stride, j0 = 4 * at - lead;
+    float4 q = make_float4(CUDART_INF_F, CUDART_INF_F, CUDART_INF_F, CUDART_INF_F);
+    if (live && j0 >= 0 && j0 + 4 <= J) q = ld_plain(base + at);
+    v.x[4 * k] = -q.x;
+    v.x[4 * k + 1] = -q.y;
+    v.x[4 * k + 2] = -q.z;
+    v.x[4 * k + 3] = -q.w;
+  }
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int j0 = 4 * (first + k * stride) - lead;
+    if (live && (j0 < 0 || j0 + 4 > J) && j0 < J) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (j0 + c >= 0 && j0 + c < J) v.x[4 * k + c] = -ld_plain(row + j0 + c);
+    }
+  }
+  return v;
+}
+
+// to[j] = x, less `hot` at the label; the values are where load_row of `row` has put them, and `to` may lie otherwise to 16 bytes
+template <int NV>
+__device__ __forceinline__ void store_row(float* to, const float* row, const RowValues<NV>& v, int J, long long label, float hot, int first,
+                                          int stride) {
+  const int lead = (int)(((uintptr_t)row >> 2) & 3);
+  const bool alike = (((uintptr_t)to ^ (uintptr_t)row) & 15) == 0;
+  float4* base = (float4*)(to - lead);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) {
+    const int at = first + k * stride, j0 = 4 * at - lead;
+    float q[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) q[c] = v.x[4 * k + c] - (j0 + c == label ? hot : 0.f);
+    if (alike && j0 >= 0 && j0 + 4 <= J) {
+      base[at] = make_float4(q[0], q[1], q[2], q[3]);
+    } else if (j0 < J) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (j0 + c >= 0 && j0 + c < J) to[j0 + c] = q[c];
+    }
+  }
+}
+
+template <int W>
+__device__ __forceinline__ float lanes_max(float m) {
+#pragma unroll
+  for (int d = W / 2; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  return m;
+}
+template <int W>
+__device__ __forceinline__ float lanes_sum(float s) {
+#pragma unroll
+  for (int d = W / 2; d >= 1; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  return s;
+}
+
+struct RowOut {
+  float* logp;
+  double* logp64;
+  float2* stats;
+  float* factor;
+};
+struct Policy {
+  const float *old, *adv, *ref;
+  const double* inv_n;
+  double3* terms;
+  float* dz;           // null: no gradient wanted
+  PolicyParams q;
+};
+
+// the numbers of one row, written by one thread; returns the gradient's factor
+__device__ __forceinline__ float row_numbers(long long r, bool live, float z_label, float2 st, const RowOut& out, const Policy& pol, bool policy,
+                                             bool writes) {
+  const double lp = live ? label_logp(z_label, st) : 0.0;
+  float f = 0.f;
+  if (policy) {
+    double3 term = make_double3(0, 0, 0);
+    if (live) {
+      const PolicyRow p = policy_row(lp, ld_plain(pol.old + r), ld_plain(pol.adv + r), pol.ref != nullptr,
+                                     pol.ref ? ld_plain(pol.ref + r) : 0.f, pol.q);
+      f = (float)(p.slope * ld_plain(pol.inv_n));
+      term = make_double3(p.loss, p.kl, p.clipped ? 1.0 : 0.0);
+    }
+    if (writes) pol.terms[r] = term;
+  }
+  if (writes) {
+    if (out.logp) out.logp[r] = (float)lp;
+    if (out.logp64) out.logp64[r] = lp;
+    if (out.stats) out.stats[r] = st;
+    if (out.factor) out.factor[r] = f;
+  }
+  return f;
+}
+
+// T threads; G lanes to a row, up to a warp, or G = T: a CTA, or with CLUSTER all CTAs of a cluster
+template <int T, int G, int NV, bool CLUSTER, bool POLICY>
+__global__ void __launch_bounds__(T, G == T && NV == 8 ? 1024 / T : 1)
+choice_rows_kernel(const float* z, const long long* labels, RowOut out, Policy pol, long long R, int J) {
+  chain_wait();
+  chain_next();
+  constexpr int W = G < 32 ? G : 32;
+  const int gl = threadIdx.x % G, lane = threadIdx.x & 31;
+  int rank = 0, ctas = 1;
+  if (CLUSTER) {
+    rank = (int)cg::this_cluster().block_rank();
+    ctas = (int)cg::this_cluster().num_blocks();
+  }
+  const long long r = G == T ? (long long)(blockIdx.x / ctas) : (long long)blockIdx.x * (T / G) + threadIdx.x / G;
+  const bool ok = r < R;                       // (of whole groups; all lanes run the shuffles)
+  const long long label = ok ? ld_plain(labels + r) : -1;
+  const bool live = counts(label, J);
+  const float* row = z + (ok ? r : 0) * J;
+  const int first = rank * G * NV + gl;
+  RowValues<NV> v = load_row<NV>(row, J, live, first, G);
+  const float z_label = live ? ld_plain(row + label) : 0.f;
+  float m[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX}, s[4] = {};
+#pragma unroll
+  for (int k = 0; k < 4 * NV; ++k) m[k % 4] = fmaxf(m[k % 4], v.x[k]);
+  const float mine = lanes_max<W>(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+#pragma unroll
+  for (int k = 0; k < 4 * NV; ++k) {
+    v.x[k] = exp_term(v.x[k] - mine);
+    s[k % 4] += v.x[k];
+  }
+  float top = mine, total = lanes_sum<W>((s[0] + s[1]) + (s[2] + s[3]));
+  float f;
+  if (G == T) {
+    __shared__ float2 part[32];
+    __shared__ float2 cta;
+    __shared__ float factor;
+    if (lane == 0) part[threadIdx.x >> 5] = make_float2(top, total);
+    __syncthreads();
+    float2 p = lane < T / 32 ? part[lane] : make_float2(-FLT_MAX, 0.f);
+    top = lanes_max<32>(p.x);
+    total = lanes_sum<32>(p.y * exp_term(p.x - top));
+    if (CLUSTER) {
+      cg::cluster_group cl = cg::this_cluster();
+      if (threadIdx.x == 0) cta = make_float2(top, total);
+      cl.sync();
+      p = lane < ctas ? *cl.map_shared_rank(&cta, lane) : make_float2(-FLT_MAX, 0.f);
+      top = lanes_max<32>(p.x);
+      total = lanes_sum<32>(p.y * exp_term(p.x - top));
+      cl.sync();                               // no CTA leaves while its numbers may still be read
+    }
+    if (threadIdx.x == 0) factor = row_numbers(r, live, z_label, make_float2(top, total), out, pol, POLICY, rank == 0);
+    if (!POLICY) return;
+    __syncthreads();
+    f = factor;
+  } else {
+    f = row_numbers(r, live, z_label, make_float2(top, total), out, pol, POLICY, ok && gl == 0);
+  }
+  if (!POLICY || pol.dz == nullptr || !ok) return;
+  const float scale = f * (exp_term(mine - top) / total);
+#pragma unroll
+  for (int k = 0; k < 4 * NV; ++k) v.x[k] = f == 0.f ? 0.f : v.x[k] * scale;
+  store_row<NV>(pol.dz + r * J, row, v, J, label, f, first, G);
+}
+
+// Rows longer than a cluster's registers: a CTA of T threads per row goes through it once for the sums, by element, and once more for
+// the gradient.
+template <int T, bool POLICY>
+__global__ void __launch_bounds__(T)
+choice_long_rows_kernel(const float* z, const long long* labels, RowOut out, Policy pol, long long R, int J) {
+  chain_wait();
+  chain_next();
+  __shared__ float2 part[32];
+  __shared__ float factor;
+  const long long r = blockIdx.x;
+  const long long label = ld_plain(labels + r);
+  const bool live = counts(label, J);
+  const float* row = z + r * J;
+  float top = -FLT_MAX, total = 0.f;
+  if (live)
+    for (int j0 = threadIdx.x; j0 < J; j0 += 4 * T) {
+      float x[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[c] = j0 + c * T < J ? -ld_plain(row + j0 + c * T) : -CUDART_INF_F;
+      const float t = fmaxf(fmaxf(top, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
+      total = total * exp_term(top - t) + ((exp_term(x[0] - t) + exp_term(x[1] - t)) + (exp_term(x[2] - t) + exp_term(x[3] - t)));
+      top = t;
+    }
+  float t = lanes_max<32>(top);
+  total = lanes_sum<32>(total * exp_term(top - t));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_float2(t, total);
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  const float2 p = lane < T / 32 ? part[lane] : make_float2(-FLT_MAX, 0.f);
+  top = lanes_max<32>(p.x);
+  total = lanes_sum<32>(p.y * exp_term(p.x - top));
+  if (threadIdx.x == 0) factor = row_numbers(r, live, live ? ld_plain(row + label) : 0.f, make_float2(top, total), out, pol, POLICY, true);
+  if (!POLICY || pol.dz == nullptr) return;
+  __syncthreads();
+  const float f = factor, scale = f / total;
+  float* to = pol.dz + r * J;
+  for (int j = threadIdx.x; j < J; j += T)
+    to[j] = f == 0.f ? 0.f : exp_term(-ld_plain(row + j) - top) * scale - (j == label ? f : 0.f);
+}
+
+// dz = factor * (p - onehot), from the kept (top, total): no sums, so a row is cut into chunks of a CTA where it is long. From the last
+// row to the first: the forward has gone the other way, and what it read last may still be in L2.
+template <int T, int G, int NV>
+__global__ void __launch_bounds__(T)
+choice_grad_kernel(const float* z, const long long* labels, const float2* stats, const float* factor, const float* gout,
+                   float* __restrict__ dz, long long R, int J, int chunks) {
+  chain_wait();
+  chain_next();
+  const int gl = threadIdx.x % G;
+  const long long back = G == T ? (long long)(blockIdx.x / chunks) : (long long)blockIdx.x * (T / G) + threadIdx.x / G;
+  if (back >= R) return;
+  const long long r = R - 1 - back;
+  const int first = (G == T ? (int)(blockIdx.x % chunks) * G * NV : 0) + gl;
+  const long long label = ld_plain(labels + r);
+  const float f = ld_plain(factor + r) * (gout ? ld_plain(gout) : 1.f);
+  const bool live = counts(label, J) && f != 0.f;
+  const float2 st = ld_plain(stats + r);
+  RowValues<NV> v = load_row<NV>(z + r * J, J, live, first, G);
+  const float scale = live ? f / st.y : 0.f;
+#pragma unroll
+  for (int k = 0; k < 4 * NV; ++k) v.x[k] = live ? exp_term(v.x[k] - st.x) * scale : 0.f;
+  store_row<NV>(dz + r * J, z + r * J, v, J, label, live ? f : 0.f, first, G);
+}
+
+// dz *= *gout, unless that is 1 (the loss is the whole objective): then there is nothing to do
+__global__ void __launch_bounds__(256) scale_kernel(float* dz, const float* gout, size_t n) {
+  chain_wait();
+  chain_next();
+  const float g = ld_plain(gout);
+  if (g == 1.f) return;
+  const size_t stride = (size_t)gridDim.x * 256;
+  for (size_t e = (size_t)blockIdx.x * 256 + threadIdx.x; e < n; e += stride) dz[e] *= g;
 }
 
 // rows [first, last) of a text; whatever the caller's numbers are, inside [0, R)
@@ -235,12 +446,59 @@ int check_rows(long long R, int J) {
   return R > 0x7fffffffLL ? SNNTC_E_TOO_LARGE : SNNTC_OK;
 }
 
-int launch_rows(const float* z, const long long* labels, float* logp, double* logp64, float* stats, float* factor, long long R, int J,
-                cudaStream_t s) {
-  const unsigned grid = (unsigned)((R * 32 + kRowThreads - 1) / kRowThreads);
-  (void)launch_chained(choice_rows_kernel, grid, kRowThreads, 0, s, 0, z, labels, logp, logp64, (float2*)stats, factor, R, J);
+// Longest row whose covering vectors fit `lanes` lanes of nv: rows that all start on 16 bytes fill them, others may begin three
+// elements into the first
+struct RowShape {
+  int J, slack;
+  RowShape(const float* z, int J) : J(J), slack((uintptr_t)z % 16 == 0 && J % 4 == 0 ? 0 : 3) {}
+  bool fits(int lanes, int nv) const { return J + slack <= 4 * lanes * nv; }
+};
+
+template <int T, int G, int NV, bool POLICY>
+int launch_rows_as(unsigned cluster, const float* z, const long long* labels, const RowOut& out, const Policy& pol, long long R, int J,
+                   cudaStream_t s) {
+  if constexpr (G == T) {
+    if (cluster > 1) {
+      (void)launch_chained(choice_rows_kernel<T, G, NV, true, POLICY>, (unsigned)R * cluster, T, 0, s, cluster, z, labels, out, pol, R, J);
+      return done();
+    }
+  }
+  const unsigned grid = G == T ? (unsigned)R : (unsigned)((R + T / G - 1) / (T / G));
+  (void)launch_chained(choice_rows_kernel<T, G, NV, false, POLICY>, grid, T, 0, s, 0, z, labels, out, pol, R, J);
   return done();
 }
+
+template <bool POLICY>
+int launch_rows(const float* z, const long long* labels, const RowOut& out, const Policy& pol, long long R, int J, cudaStream_t s) {
+  const RowShape w(z, J);
+  if (w.fits(4, 1)) return launch_rows_as<256, 4, 1, POLICY>(1, z, labels, out, pol, R, J, s);
+  if (w.fits(8, 1)) return launch_rows_as<256, 8, 1, POLICY>(1, z, labels, out, pol, R, J, s);
+  if (w.fits(16, 1)) return launch_rows_as<256, 16, 1, POLICY>(1, z, labels, out, pol, R, J, s);
+  if (w.fits(32, 1)) return launch_rows_as<256, 32, 1, POLICY>(1, z, labels, out, pol, R, J, s);
+  if (w.fits(32, 2)) return launch_rows_as<256, 32, 2, POLICY>(1, z, labels, out, pol, R, J, s);
+  if (w.fits(32, 4)) return launch_rows_as<256, 32, 4, POLICY>(1, z, labels, out, pol, R, J, s);
+  if (w.fits(32, 8)) return launch_rows_as<256, 32, 8, POLICY>(1, z, labels, out, pol, R, J, s);
+  if (w.fits(128, 4)) return launch_rows_as<128, 128, 4, POLICY>(1, z, labels, out, pol, R, J, s);
+  if (w.fits(256, 4)) return launch_rows_as<256, 256, 4, POLICY>(1, z, labels, out, pol, R, J, s);
+  if (w.fits(256, 8)) return launch_rows_as<256, 256, 8, POLICY>(1, z, labels, out, pol, R, J, s);
+  for (unsigned cluster = 1; cluster <= 8; cluster *= 2)
+    if (w.fits(512 * (int)cluster, 8)) return launch_rows_as<512, 512, 8, POLICY>(cluster, z, labels, out, pol, R, J, s);
+  (void)launch_chained(choice_long_rows_kernel<512, POLICY>, (unsigned)R, 512, 0, s, 0, z, labels, out, pol, R, J);
+  return done();
+}
+
+template <int T, int G, int NV>
+int launch_grad_as(const float* z, const long long* labels, const float* stats, const float* factor, const float* gout, float* dz,
+                   long long R, int J, cudaStream_t s) {
+  const int chunks = G == T ? (int)(((long long)J + 3 + 4 * T * NV - 1) / (4 * T * NV)) : 1;
+  const long long grid = G == T ? R * chunks : (R + T / G - 1) / (T / G);
+  if (grid > 0x7fffffffLL) return SNNTC_E_TOO_LARGE;
+  (void)launch_chained(choice_grad_kernel<T, G, NV>, (unsigned)grid, T, 0, s, 0, z, labels, (const float2*)stats, factor, gout, dz, R, J, chunks);
+  return done();
+}
+
+// One cluster of up to eight CTAs
+unsigned sum_ctas(long long n) { return n >= 8LL * kSumThreads ? 8 : (unsigned)((n + kSumThreads - 1) / kSumThreads); }
 
 }  // namespace
 
@@ -249,33 +507,48 @@ extern "C" {
 int snntc_label_logp_forward(const float* z, const long long* labels, float* logp, float* stats_2R, long long R, int J, void* stream) {
   if (!z || !labels || !logp) return SNNTC_E_NULL;
   if (const int rc = check_rows(R, J)) return rc;
-  return launch_rows(z, labels, logp, nullptr, stats_2R, nullptr, R, J, (cudaStream_t)stream);
+  return launch_rows<false>(z, labels, RowOut{logp, nullptr, (float2*)stats_2R, nullptr}, Policy{}, R, J, (cudaStream_t)stream);
 }
 
 int snntc_choice_backward(const float* z, const long long* labels, const float* stats_2R, const float* factor, const float* gout,
                           float* dz, long long R, int J, void* stream) {
   if (!z || !labels || !stats_2R || !factor || !dz) return SNNTC_E_NULL;
   if (const int rc = check_rows(R, J)) return rc;
-  const unsigned grid = (unsigned)((R * 32 + kRowThreads - 1) / kRowThreads);
-  (void)launch_chained(choice_grad_kernel, grid, kRowThreads, 0, (cudaStream_t)stream, 0, z, labels, (const float2*)stats_2R, factor, gout,
-                       dz, R, J);
-  return done();
+  cudaStream_t s = (cudaStream_t)stream;
+  const RowShape w(z, J);
+  if (w.fits(4, 1)) return launch_grad_as<256, 4, 1>(z, labels, stats_2R, factor, gout, dz, R, J, s);
+  if (w.fits(16, 1)) return launch_grad_as<256, 16, 1>(z, labels, stats_2R, factor, gout, dz, R, J, s);
+  if (w.fits(32, 2)) return launch_grad_as<256, 32, 2>(z, labels, stats_2R, factor, gout, dz, R, J, s);
+  if (w.fits(32, 4)) return launch_grad_as<256, 32, 4>(z, labels, stats_2R, factor, gout, dz, R, J, s);
+  return launch_grad_as<256, 256, 4>(z, labels, stats_2R, factor, gout, dz, R, J, s);
 }
 
-size_t snntc_policy_loss_workspace_bytes(long long R) { return R <= 0 ? 0 : (size_t)R * sizeof(double); }
+size_t snntc_policy_loss_workspace_bytes(long long R) { return R <= 0 ? 0 : (size_t)R * sizeof(double3) + 256; }
 
 int snntc_policy_loss(const float* z, const long long* labels, const float* old_logp, const float* advantage, const float* ref_logp,
-                      float* loss, float* kl_and_clipped, float* stats_2R, float* factor, long long R, int J, double clip_low,
-                      double clip_high, double kl_coef, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!z || !labels || !old_logp || !advantage || !loss || !kl_and_clipped || !stats_2R || !factor) return SNNTC_E_NULL;
+                      float* loss, float* kl_and_clipped, float* stats_2R, float* factor, float* dz, long long R, int J,
+                      double clip_low, double clip_high, double kl_coef, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!z || !labels || !old_logp || !advantage || !loss || !kl_and_clipped) return SNNTC_E_NULL;
   if (const int rc = check_rows(R, J)) return rc;
   if (!(clip_low >= 0 && clip_low <= 1 && clip_high >= 0 && kl_coef - kl_coef == 0) || (kl_coef != 0 && !ref_logp)) return SNNTC_E_PARAMS;
   if (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < snntc_policy_loss_workspace_bytes(R)) return SNNTC_E_WORKSPACE;
-  double* lp = (double*)workspace;
+  double* inv_n = (double*)workspace;
+  double3* terms = (double3*)((char*)workspace + 256);
   cudaStream_t s = (cudaStream_t)stream;
-  if (const int rc = launch_rows(z, labels, nullptr, lp, stats_2R, factor, R, J, s)) return rc;
-  const PolicyParams q{1 - clip_low, 1 + clip_high, kl_coef};
-  (void)launch_chained(policy_rows_kernel, 1, 1024, 0, s, 0, lp, labels, old_logp, advantage, ref_logp, factor, loss, kl_and_clipped, R, J, q);
+  const unsigned ctas = sum_ctas(R);
+  (void)launch_chained(policy_count_kernel, ctas, kSumThreads, 0, s, ctas, labels, inv_n, R, J);
+  if (const int rc = done()) return rc;
+  const Policy pol{old_logp, advantage, ref_logp, inv_n, terms, dz, PolicyParams{1 - clip_low, 1 + clip_high, kl_coef}};
+  if (const int rc = launch_rows<true>(z, labels, RowOut{nullptr, nullptr, (float2*)stats_2R, factor}, pol, R, J, s)) return rc;
+  (void)launch_chained(policy_mean_kernel, ctas, kSumThreads, 0, s, ctas, terms, inv_n, loss, kl_and_clipped, R);
+  return done();
+}
+
+int snntc_scale_gradient(float* dz, const float* gout, size_t n, void* stream) {
+  if (!dz || !gout) return SNNTC_E_NULL;
+  if (n == 0) return SNNTC_OK;
+  const size_t ctas = (n + 1023) / 1024;
+  (void)launch_chained(scale_kernel, (unsigned)(ctas < 1184 ? ctas : 1184), 256, 0, (cudaStream_t)stream, 0, dz, gout, n);
   return done();
 }
 
@@ -294,7 +567,7 @@ int snntc_preference_loss(const float* z, const long long* labels, const long lo
   double* lp = (double*)workspace;
   double* terms = lp + R;
   cudaStream_t s = (cudaStream_t)stream;
-  if (const int rc = launch_rows(z, labels, nullptr, lp, stats_2R, factor, R, J, s)) return rc;
+  if (const int rc = launch_rows<false>(z, labels, RowOut{nullptr, lp, (float2*)stats_2R, factor}, Policy{}, R, J, s)) return rc;
   (void)launch_chained(preference_pairs_kernel, (unsigned)P, 512, 0, s, 0, lp, starts, ref_logp, margins, factor, terms, R, P,
                        R / (2LL * P), beta, smoothing);
   if (const int rc = done()) return rc;

@@ -715,32 +715,46 @@ struct ChoiceState : torch::CustomClassHolder {
   int P = 0;          // pairs; 0: a policy loss
   const char* name() const { return P ? "preference_loss" : "policy_loss"; }
 };
-struct ChoiceLoss { Tensor loss, more, stats, factor; };   // more: [KL term, clipped] or the margins
+// more: [KL term, clipped] or the margins; kept: (top, total) and the factor of every row; dz: the gradient, of a policy loss
+struct ChoiceLoss { Tensor loss, more, kept, dz; };
 
-ChoiceLoss choice_loss_call(const ChoiceState& s) {
+ChoiceLoss choice_loss_call(const ChoiceState& s, bool grad) {
   const Rows& r = s.rows;
   const c10::cuda::CUDAGuard guard(r.z.device());
   ChoiceLoss o;
   o.loss = empty_like_dev({}, r.z);
   o.more = empty_like_dev({s.P ? s.P : 2}, r.z);
-  o.stats = empty_like_dev({r.R, 2}, r.z);
-  o.factor = empty_like_dev({r.R}, r.z);
+  if (grad || s.P) o.kept = empty_like_dev({3 * r.R}, r.z);
+  if (grad && !s.P) o.dz = empty_like_dev(r.z.sizes(), r.z);
+  float* stats = ptr(o.kept);
+  float* factor = stats ? stats + 2 * r.R : nullptr;
   const size_t bytes = s.P ? snntc_preference_loss_workspace_bytes(r.R, s.P) : snntc_policy_loss_workspace_bytes(r.R);
   const Tensor ws = workspace(bytes, r.z);
   const int rc = s.P ? snntc_preference_loss(ptr(r.z), labels_of(r.label), s.starts.defined() ? labels_of(s.starts) : nullptr, ptr(s.ref_logp),
-                                             ptr(o.loss), ptr(o.more), ptr(o.stats), ptr(o.factor), r.R, r.J, s.P, s.a, s.b, ws.data_ptr(),
-                                             bytes, stream_of(r.z))
+                                             ptr(o.loss), ptr(o.more), stats, factor, r.R, r.J, s.P, s.a, s.b, ws.data_ptr(), bytes,
+                                             stream_of(r.z))
                      : snntc_policy_loss(ptr(r.z), labels_of(r.label), ptr(s.old_logp), ptr(s.advantage), ptr(s.ref_logp), ptr(o.loss),
-                                         ptr(o.more), ptr(o.stats), ptr(o.factor), r.R, r.J, s.a, s.b, s.c, ws.data_ptr(), bytes, stream_of(r.z));
+                                         ptr(o.more), stats, factor, ptr(o.dz), r.R, r.J, s.a, s.b, s.c, ws.data_ptr(), bytes,
+                                         stream_of(r.z));
   check(rc, s.name());
   return o;
 }
 
+// The gradient that a policy loss formed with its value. The first backward hands it out, scaled by the incoming gradient; autograd
+// may add to it in place or keep it as somebody's .grad, so a second backward over the same graph forms one of its own.
+struct KeptGradient : torch::CustomClassHolder {
+  std::mutex mutex;
+  Tensor dz;
+};
+
 struct ChoiceLossFunction : torch::autograd::Function<ChoiceLossFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& logit, c10::intrusive_ptr<ChoiceState> s) {
-    const ChoiceLoss o = choice_loss_call(*s);
-    ctx->save_for_backward({s->rows.z, s->rows.label, o.stats, o.factor});
+    const ChoiceLoss o = choice_loss_call(*s, true);
+    auto k = c10::make_intrusive<KeptGradient>();
+    k->dz = o.dz;
+    ctx->save_for_backward({s->rows.z, s->rows.label, o.kept});
     ctx->saved_data["pairs"] = (int64_t)s->P;
+    ctx->saved_data["gradient"] = c10::IValue::make_capsule(k);
     ctx->mark_non_differentiable({o.more});
     return {o.loss, o.more};
   }
@@ -749,7 +763,19 @@ struct ChoiceLossFunction : torch::autograd::Function<ChoiceLossFunction> {
     const char* what = ctx->saved_data["pairs"].toInt() ? "preference_loss" : "policy_loss";
     check_backward(saved[0], what);
     const Tensor g = as_cuda_f32(grads[0], "gradient of the loss");
-    return {choice_backward(saved[0], saved[1], saved[2], saved[3], g, what), Tensor()};
+    const auto k = c10::static_intrusive_pointer_cast<KeptGradient>(ctx->saved_data["gradient"].toCapsule());
+    Tensor dz;
+    {
+      const std::lock_guard<std::mutex> lock(k->mutex);
+      std::swap(dz, k->dz);
+    }
+    if (!dz.defined()) {
+      const int64_t R = saved[1].numel();
+      return {choice_backward(saved[0], saved[1], saved[2].narrow(0, 0, 2 * R), saved[2].narrow(0, 2 * R, R), g, what), Tensor()};
+    }
+    const c10::cuda::CUDAGuard guard(dz.device());
+    check(snntc_scale_gradient(ptr(dz), ptr(g), (size_t)dz.numel(), stream_of(dz)), what);
+    return {dz, Tensor()};
   }
 };
 
@@ -758,7 +784,7 @@ std::pair<Tensor, Tensor> choice_loss(const Tensor& logit, c10::intrusive_ptr<Ch
     auto r = ChoiceLossFunction::apply(logit, s);
     return {r[0], r[1]};
   }
-  const ChoiceLoss o = choice_loss_call(*s);
+  const ChoiceLoss o = choice_loss_call(*s, false);
   return {o.loss, o.more};
 }
 

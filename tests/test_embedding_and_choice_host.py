@@ -38,14 +38,16 @@ def test_status_codes_of_the_losses_on_choices():
         a[k] = 0
         assert lib.snntc_choice_backward(*a, 4, 3, 0) == -1
     assert lib.snntc_choice_backward(*args, 0, 3, 0) == -2
-    pol = lambda p=(FAKE,) * 9, R=4, J=3, lo=0.2, hi=0.2, kl=0.1, ws=FAKE, n=1 << 40: lib.snntc_policy_loss(*p, R, J, lo, hi, kl, ws, n, 0)  # noqa: E731
-    for k in (0, 1, 2, 3, 5, 6, 7, 8):
-        p = [FAKE] * 9
+    assert lib.snntc_scale_gradient(0, FAKE, 4, 0) == lib.snntc_scale_gradient(FAKE, 0, 4, 0) == -1
+    assert lib.snntc_scale_gradient(FAKE, FAKE, 0, 0) == 0
+    pol = lambda p=(FAKE,) * 10, R=4, J=3, lo=0.2, hi=0.2, kl=0.1, ws=FAKE, n=1 << 40: lib.snntc_policy_loss(*p, R, J, lo, hi, kl, ws, n, 0)  # noqa: E731
+    for k in (0, 1, 2, 3, 5, 6):
+        p = [FAKE] * 10
         p[k] = 0
         assert pol(p) == -1
     assert pol(R=0) == pol(J=0) == -2
     assert pol(lo=-0.1) == pol(lo=1.1) == pol(hi=-0.1) == pol(lo=float("nan")) == pol(kl=float("inf")) == -8
-    assert pol([FAKE] * 4 + [0] + [FAKE] * 4) == -8                          # a KL term without a reference
+    assert pol([FAKE] * 4 + [0] + [FAKE] * 5) == -8                          # a KL term without a reference
     assert pol(ws=0) == pol(ws=FAKE + 8) == pol(n=lib.snntc_policy_loss_workspace_bytes(4) - 1) == -5
     pre = lambda p=(FAKE,) * 8, R=8, J=3, P=2, beta=0.1, eps=0.0, ws=FAKE, n=1 << 40: lib.snntc_preference_loss(*p, R, J, P, beta, eps, ws, n, 0)  # noqa: E731
     for k in (0, 1, 4, 5, 6, 7):

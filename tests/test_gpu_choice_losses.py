@@ -2,10 +2,10 @@
 evaluations of their formulas.
 
 Tolerances, with u = 2^-24 (half a step of float32), d_j = -z_j - max(-z): a term exp(d_j) of a row's sum is off by the rounding of
-d_j and of its product with log2(e), 2 |d_j| u, and by the exponential's own 2^-22 = 4 u at most; the sum of a row by its longest chain of
+d_j, of log2(e) and of their product, 2.5 |d_j| u, and by the exponential's own 2^-22 = 4 u at most; the sum of a row by its longest chain of
 additions, 64 u for the row lengths here (a lane adds at most 32 and the tree over lanes has 10 levels), which weights the terms'
-errors by p_j. So total is off by REL = (4 + 64 + 2 sum_j p_j |d_j|) u relative, lp by REL + |lp| u (its own rounding),
-p_j by REL + (2 |d_j| + 4 + 2) u relative, and a gradient factor * (p - onehot) by |factor| (p_j * that + 2 u) where factor is exact."""
+errors by p_j. So total is off by REL = (4 + 64 + 2.5 sum_j p_j |d_j|) u relative, lp by REL + |lp| u (its own rounding),
+p_j by REL + (2.5 |d_j| + 4 + 3) u relative, and a gradient factor * (p - onehot) by |factor| (p_j * that + 2 u) where factor is exact."""
 import math
 
 import pytest
@@ -39,22 +39,22 @@ class Ref:
         self.lp = torch.where(self.counts, torch.log_softmax(x, 1).gather(1, at[:, None])[:, 0], 0.0)
         self.p = torch.softmax(x, 1)
         d = (x.amax(1, keepdim=True) - x).clamp(max=200.0)          # (beyond that p is 0 on both sides)
-        self.rel = (68 + 2 * (self.p * d).sum(1)) * U
-        self.p_rel = self.rel[:, None] + (2 * d + 6) * U
+        self.rel = (68 + 2.5 * (self.p * d).sum(1)) * U
+        self.p_rel = self.rel[:, None] + (2.5 * d + 7) * U
         self.hot = torch.zeros_like(self.p)
         self.hot[torch.arange(R, device=z.device), at] = 1.0
 
     def check_lp(self, lp):
         assert ((lp.double() - self.lp).abs() <= self.counts * (self.rel + self.lp.abs() * U) * 1.001).all()
 
-    def check_grad(self, grad, factor, factor_tol):
-        """factor: float64 per row; factor_tol: how far the kernel's may be off"""
+    def check_grad(self, grad, factor, factor_tol, times=1):
+        """factor: float64 per row; factor_tol: how far the kernel's may be off; times: grad is a sum with so many gradients' errors"""
         import torch
         factor, factor_tol = torch.where(self.counts, factor, 0.0)[:, None], torch.where(self.counts, factor_tol, 0.0)[:, None]
         want = factor * (self.p - self.hot)
         tol = factor.abs() * (self.p * self.p_rel + 2 * U * (self.p + self.hot)) + factor_tol * (self.p + self.hot) * 1.01 + 1e-38
         err = (grad.double() - want).abs()
-        assert (err <= tol * 1.001).all(), float((err / tol).max())
+        assert (err <= times * tol * 1.001).all(), float((err / tol).max())
         assert (grad[~self.counts] == 0).all()
 
 
@@ -143,7 +143,7 @@ def test_policy_loss_and_its_gradient(R, J, with_ref):
     (again * -2.0).backward(retain_graph=True)
     assert torch.equal(z1.grad, -2.0 * first)         # (a power of two moves no rounding)
     again.backward()
-    assert torch.allclose(z1.grad, -first, rtol=1e-6, atol=1e-30)
+    ref.check_grad(-z1.grad, want["factor"], want["factor_tol"], times=4)      # -2 of the first, one of its own; the last is the sum's rounding
     with torch.no_grad():
         alone = train.policy_loss(z1, lab, old, adv, ref_logp=refp, clip_low=0.2, clip_high=0.25, kl_coef=kl_coef, with_stats=True)
     assert torch.equal(alone[0], loss) and torch.equal(alone[1], stats)
@@ -365,7 +365,8 @@ def test_strides_offsets_and_leading_dimensions():
             b.backward()
             assert torch.allclose(a, b, rtol=1e-5) and torch.allclose(moved.grad, zz.grad, rtol=1e-5, atol=1e-9)
     zl, ll = z.view(3, 4, 5, 33), lab.view(3, 4, 5)
-    assert torch.equal(train.label_log_probs(zl.transpose(0, 1), ll.transpose(0, 1)), plain.detach().view(3, 4, 5).transpose(0, 1))
+    moved = train.label_log_probs(zl.transpose(0, 1), ll.transpose(0, 1))     # (a row's bits may go with where it starts to 16 bytes)
+    Ref(z, lab).check_lp(moved.transpose(0, 1).reshape(60))
 
 
 def test_more_than_32_bits_of_logits():
