@@ -30,13 +30,17 @@ using snntc::ld_plain;
 
 __device__ __forceinline__ bool counts(long long label, int J) { return label >= 0 && label < J; }
 
-// exp(d) for d <= 0 as 2^(d log2 e), one product and one instruction: off by 2^-22 + |d| 2^-23 relative. The terms of a row's sum
-// and its probabilities are all it is used for; what is one number per row takes exp and log in 64 bits.
+// exp(d) for d <= 0 as 2^(d log2 e), one product and one instruction: off by 2^-22 + |d| 2^-23 relative, and by some -5e-8 in the mean.
 __device__ __forceinline__ float exp_term(float d) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * 1.44269504f));
   return e;
 }
+// A term of a row's sum. Where log-probabilities are what is wanted, expf, whose mean is off by 5e-9: those of a text's rows are added
+// up, and what they have in common adds up with them (margins of 8192 rows in 32 texts: 1.3e-6 off with the short form, relative). It is
+// the dearer one: 4096 rows of 32 768 93 us, 84 with the short form, which a single row's ratio and probabilities are served by.
+template <bool SHORT>
+__device__ __forceinline__ float sum_term(float d) { return SHORT ? exp_term(d) : expf(d); }
 
 constexpr int kSumThreads = 1024;
 
@@ -110,6 +114,7 @@ policy_count_kernel(const long long* labels, double* __restrict__ inv_n, long lo
   chain_wait();
   chain_next();
   double3 n = make_double3(0, 0, 0);
+#pragma unroll 8
   for (long long r = (long long)blockIdx.x * kSumThreads + threadIdx.x; r < R; r += (long long)gridDim.x * kSumThreads)
     n.x += counts(ld_plain(labels + r), J) ? 1.0 : 0.0;
   n = cluster_sum(n);
@@ -117,11 +122,11 @@ policy_count_kernel(const long long* labels, double* __restrict__ inv_n, long lo
 }
 
 __global__ void __launch_bounds__(kSumThreads)
-policy_mean_kernel(const double3* terms, const double* inv_n, float* __restrict__ loss, float* __restrict__ out2, long long R) {
+policy_mean_kernel(const double3* terms, const double* inv_n, float* __restrict__ loss, float* __restrict__ out2, long long n) {
   chain_wait();
   chain_next();
   double3 sum = make_double3(0, 0, 0);
-  for (long long r = (long long)blockIdx.x * kSumThreads + threadIdx.x; r < R; r += (long long)gridDim.x * kSumThreads) {
+  for (long long r = (long long)blockIdx.x * kSumThreads + threadIdx.x; r < n; r += (long long)gridDim.x * kSumThreads) {
     const double3 t = ld_plain(terms + r);
     sum.x += t.x;
     sum.y += t.y;
@@ -136,7 +141,7 @@ policy_mean_kernel(const double3* terms, const double* inv_n, float* __restrict_
   }
 }
 
-// ---- rows. A group of G lanes (part of a warp, a warp, a CTA, or the CTAs of a cluster) holds a row in registers, NV vectors of four
+// ---- rows. A group of G lanes (part of a warp, a warp, a CTA) holds a row in registers, NV vectors of four
 // a lane, all loads in flight at once: the row is read from memory once, and where the loss's factor follows from the row alone
 // (the policy loss), its gradient is written in the same pass. Rows of any length start anywhere, so a row is seen through the
 // 16-byte vectors that cover it; those that stick out at its ends are loaded and stored by element.
@@ -195,6 +200,72 @@ __device__ __forceinline__ void store_row(float* to, const float* row, const Row
   }
 }
 
+// A row as its whole 16-byte vectors and the up to six elements at its ends, of which the first lanes of a group take one each
+struct Ends {
+  const float4* body;
+  int head, vectors, at;
+  bool mine;
+  __device__ __forceinline__ Ends(const float* row, int J, int gl) {
+    head = min(J, (int)((4 - ((uintptr_t)row >> 2)) & 3));
+    vectors = (J - head) / 4;
+    const int tail = head + 4 * vectors;
+    body = (const float4*)(row + head);
+    at = gl < head ? gl : tail + gl - head;
+    mine = gl < head + J - tail;
+  }
+};
+
+// to = scale * exp(-row - top), less f at the label, for the vectors [v0, v1) and, with the row's first ones, its ends; zeros where f is 0.
+// By `lanes` lanes, U vectors at a time, from the last to the first. `to` is `apart` bytes behind the row.
+template <int U>
+__device__ __forceinline__ void grad_row(const float* row, ptrdiff_t apart, const Ends& e, int v0, int v1, int gl, int lanes, float top,
+                                         float scale, float f, int hot) {
+  const bool alike = (apart & 15) == 0;
+  const auto put = [&](const float4* from, float4 q) {
+    float* to = (float*)((char*)from + apart);
+    if (alike) {
+      __stcs((float4*)to, q);
+    } else {
+      to[0] = q.x;
+      to[1] = q.y;
+      to[2] = q.z;
+      to[3] = q.w;
+    }
+  };
+  if (v0 == 0 && e.mine)
+    *(float*)((char*)(row + e.at) + apart) = f == 0.f ? 0.f : exp_term(-ld_plain(row + e.at) - top) * scale - (e.at == hot ? f : 0.f);
+  if (f == 0.f) {
+    for (int b = v0 + gl; b < v1; b += lanes) put(e.body + b, make_float4(0.f, 0.f, 0.f, 0.f));
+    return;
+  }
+  const int hot_v = (hot - e.head) >> 2;
+  const float4* at = e.body + (v1 - 1 - gl);
+  for (int b = v1 - 1 - gl; b >= v0; b -= U * lanes, at -= U * lanes) {
+    float4 q[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      q[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (b - k * lanes >= v0) q[k] = __ldcs(at - k * lanes);
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (b - k * lanes < v0) break;
+      q[k].x = exp_term(-q[k].x - top) * scale;
+      q[k].y = exp_term(-q[k].y - top) * scale;
+      q[k].z = exp_term(-q[k].z - top) * scale;
+      q[k].w = exp_term(-q[k].w - top) * scale;
+      if (b - k * lanes == hot_v) {
+        const int c = (hot - e.head) & 3;
+        q[k].x -= c == 0 ? f : 0.f;
+        q[k].y -= c == 1 ? f : 0.f;
+        q[k].z -= c == 2 ? f : 0.f;
+        q[k].w -= c == 3 ? f : 0.f;
+      }
+      put(at - k * lanes, q[k]);
+    }
+  }
+}
+
 template <int W>
 __device__ __forceinline__ float lanes_max(float m) {
 #pragma unroll
@@ -222,137 +293,186 @@ struct Policy {
   PolicyParams q;
 };
 
-// the numbers of one row, written by one thread; returns the gradient's factor
-__device__ __forceinline__ float row_numbers(long long r, bool live, float z_label, float2 st, const RowOut& out, const Policy& pol, bool policy,
-                                             bool writes) {
-  const double lp = live ? label_logp(z_label, st) : 0.0;
+// What a row's numbers are formed from besides its sums: asked for when the row is, into L1, and loaded when they are needed -- in
+// registers meanwhile they would cost the row's loop its place (32 a thread at 2048 threads an SM).
+struct RowIn { float z_label, old, adv, ref; double inv_n; };
+__device__ __forceinline__ void prefetch(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(__cvta_generic_to_global(p))); }
+template <bool POLICY>
+__device__ __forceinline__ void prefetch_inputs(long long r, const float* row, long long label, const Policy& pol) {
+  prefetch(row + label);
+  if (POLICY) {
+    prefetch(pol.old + r);
+    prefetch(pol.adv + r);
+    if (pol.ref) prefetch(pol.ref + r);
+  }
+}
+template <bool POLICY>
+__device__ __forceinline__ RowIn row_inputs(long long r, bool live, const float* row, long long label, const Policy& pol) {
+  RowIn in = {};
+  if (live) {
+    in.z_label = ld_plain(row + label);
+    if (POLICY) {
+      in.old = ld_plain(pol.old + r);
+      in.adv = ld_plain(pol.adv + r);
+      if (pol.ref) in.ref = ld_plain(pol.ref + r);
+      in.inv_n = ld_plain(pol.inv_n);
+    }
+  }
+  return in;
+}
+
+// The numbers of a row, by one thread; returns the gradient's factor. ROWS rows of a CTA together: their terms of the loss are added in
+// a fixed order and leave as one (threads without a row take part in that).
+template <bool POLICY, int ROWS>
+__device__ __forceinline__ float row_numbers(const float* z, const long long* labels, long long r, bool ok, int J, float2 st, const RowOut& out,
+                                             const Policy& pol) {
+  const long long label = ok ? ld_plain(labels + r) : -1;
+  const bool live = counts(label, J);
+  const RowIn in = row_inputs<POLICY>(r, live, z + (ok ? r : 0) * J, label, pol);
+  double lp = 0.0;
   float f = 0.f;
-  if (policy) {
-    double3 term = make_double3(0, 0, 0);
-    if (live) {
-      const PolicyRow p = policy_row(lp, ld_plain(pol.old + r), ld_plain(pol.adv + r), pol.ref != nullptr,
-                                     pol.ref ? ld_plain(pol.ref + r) : 0.f, pol.q);
-      f = (float)(p.slope * ld_plain(pol.inv_n));
+  double3 term = make_double3(0, 0, 0);
+  if (live) {
+    lp = label_logp(in.z_label, st);
+    if (POLICY) {
+      const PolicyRow p = policy_row(lp, in.old, in.adv, pol.ref != nullptr, in.ref, pol.q);
+      f = (float)(p.slope * in.inv_n);
       term = make_double3(p.loss, p.kl, p.clipped ? 1.0 : 0.0);
     }
-    if (writes) pol.terms[r] = term;
   }
-  if (writes) {
+  if (ok) {
     if (out.logp) out.logp[r] = (float)lp;
     if (out.logp64) out.logp64[r] = lp;
     if (out.stats) out.stats[r] = st;
     if (out.factor) out.factor[r] = f;
   }
+  if (POLICY) {
+    if (ROWS > 32) {
+      term = block_sum(term);
+    } else if (ROWS > 1) {
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1) {
+        term.x += __shfl_xor_sync(0xffffffffu, term.x, d);
+        term.y += __shfl_xor_sync(0xffffffffu, term.y, d);
+        term.z += __shfl_xor_sync(0xffffffffu, term.z, d);
+      }
+    }
+    if (threadIdx.x == 0) pol.terms[blockIdx.x] = term;
+  }
   return f;
 }
 
-// T threads; G lanes to a row, up to a warp, or G = T: a CTA, or with CLUSTER all CTAs of a cluster
-template <int T, int G, int NV, bool CLUSTER, bool POLICY>
-__global__ void __launch_bounds__(T, G == T && NV == 8 ? 1024 / T : 1)
+// T threads with T / G rows, G lanes to a row: part of a warp, a warp, or the whole CTA.
+// HOLD: the row stays in the lanes' registers, NV vectors each; else the lanes go through it NV vectors at a time with a running
+// (maximum, sum) each, and for the policy loss once more, from the row's end to its beginning, for the gradient: what was read last is
+// still in L1 and L2.
+// The rows' numbers are formed together, by one thread a row: in 64 bits they are some 300 instructions at half rate, whether one lane
+// of a warp runs them or all (65 536 rows of 1000, a warp each: 35 of 141 us).
+template <int T, int G, int NV, bool HOLD, bool POLICY>
+__global__ void __launch_bounds__(T, HOLD ? 1024 / T : 2048 / T)
 choice_rows_kernel(const float* z, const long long* labels, RowOut out, Policy pol, long long R, int J) {
+  static_assert(G <= 32 || G == T, "a row belongs to part of a warp, a warp or the CTA");
+  constexpr int kRows = T / G, W = G < 32 ? G : 32;
+  __shared__ float2 stats[kRows > T / 32 ? kRows : T / 32];   // (top, total): of rows, or of a row's warps
+  __shared__ float factors[kRows];
   chain_wait();
   chain_next();
-  constexpr int W = G < 32 ? G : 32;
-  const int gl = threadIdx.x % G, lane = threadIdx.x & 31;
-  int rank = 0, ctas = 1;
-  if (CLUSTER) {
-    rank = (int)cg::this_cluster().block_rank();
-    ctas = (int)cg::this_cluster().num_blocks();
-  }
-  const long long r = G == T ? (long long)(blockIdx.x / ctas) : (long long)blockIdx.x * (T / G) + threadIdx.x / G;
+  const int tid = threadIdx.x, lane = tid & 31, gl = tid % G, own = tid / G;
+  const long long r0 = (long long)blockIdx.x * kRows, r = r0 + own;
   const bool ok = r < R;                       // (of whole groups; all lanes run the shuffles)
   const long long label = ok ? ld_plain(labels + r) : -1;
   const bool live = counts(label, J);
-  const float* row = z + (ok ? r : 0) * J;
-  const int first = rank * G * NV + gl;
-  RowValues<NV> v = load_row<NV>(row, J, live, first, G);
-  const float z_label = live ? ld_plain(row + label) : 0.f;
-  float m[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX}, s[4] = {};
-#pragma unroll
-  for (int k = 0; k < 4 * NV; ++k) m[k % 4] = fmaxf(m[k % 4], v.x[k]);
-  const float mine = lanes_max<W>(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
-#pragma unroll
-  for (int k = 0; k < 4 * NV; ++k) {
-    v.x[k] = exp_term(v.x[k] - mine);
-    s[k % 4] += v.x[k];
+  const float* row = z + (ok ? r : r0) * J;
+  // thread t < kRows forms the numbers of row r0 + t
+  const long long mine = r0 + tid;
+  const bool mine_ok = tid < kRows && mine < R;
+  if (mine_ok) {
+    const long long l = G == T ? label : ld_plain(labels + mine);
+    if (counts(l, J)) prefetch_inputs<POLICY>(mine, z + mine * J, l, pol);
   }
-  float top = mine, total = lanes_sum<W>((s[0] + s[1]) + (s[2] + s[3]));
-  float f;
-  if (G == T) {
-    __shared__ float2 part[32];
-    __shared__ float2 cta;
-    __shared__ float factor;
-    if (lane == 0) part[threadIdx.x >> 5] = make_float2(top, total);
-    __syncthreads();
-    float2 p = lane < T / 32 ? part[lane] : make_float2(-FLT_MAX, 0.f);
-    top = lanes_max<32>(p.x);
-    total = lanes_sum<32>(p.y * exp_term(p.x - top));
-    if (CLUSTER) {
-      cg::cluster_group cl = cg::this_cluster();
-      if (threadIdx.x == 0) cta = make_float2(top, total);
-      cl.sync();
-      p = lane < ctas ? *cl.map_shared_rank(&cta, lane) : make_float2(-FLT_MAX, 0.f);
-      top = lanes_max<32>(p.x);
-      total = lanes_sum<32>(p.y * exp_term(p.x - top));
-      cl.sync();                               // no CTA leaves while its numbers may still be read
+
+  RowValues<NV> v;
+  Ends e(row, J, gl);
+  float top = -FLT_MAX, total = 0.f;
+  if constexpr (HOLD) {
+    v = load_row<NV>(row, J, live, gl, G);
+    float m[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX}, s[4] = {};
+#pragma unroll
+    for (int k = 0; k < 4 * NV; ++k) m[k % 4] = fmaxf(m[k % 4], v.x[k]);
+    top = lanes_max<W>(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+#pragma unroll
+    for (int k = 0; k < 4 * NV; ++k) {
+      v.x[k] = sum_term<POLICY>(v.x[k] - top);
+      s[k % 4] += v.x[k];
     }
-    if (threadIdx.x == 0) factor = row_numbers(r, live, z_label, make_float2(top, total), out, pol, POLICY, rank == 0);
+    total = lanes_sum<W>((s[0] + s[1]) + (s[2] + s[3]));
+  } else {
+    if (live) {
+      for (int v0 = gl; v0 < e.vectors; v0 += NV * G) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+          float4 q = make_float4(CUDART_INF_F, CUDART_INF_F, CUDART_INF_F, CUDART_INF_F);
+          if (v0 + k * G < e.vectors) q = ld_plain(e.body + v0 + k * G);
+          v.x[4 * k] = -q.x;
+          v.x[4 * k + 1] = -q.y;
+          v.x[4 * k + 2] = -q.z;
+          v.x[4 * k + 3] = -q.w;
+        }
+        float m[4] = {top, -FLT_MAX, -FLT_MAX, -FLT_MAX}, s[4] = {};
+#pragma unroll
+        for (int k = 0; k < 4 * NV; ++k) m[k % 4] = fmaxf(m[k % 4], v.x[k]);
+        const float t = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+#pragma unroll
+        for (int k = 0; k < 4 * NV; ++k) s[k % 4] += sum_term<POLICY>(v.x[k] - t);
+        total = fmaf(total, expf(top - t), (s[0] + s[1]) + (s[2] + s[3]));
+        top = t;
+      }
+      if (e.mine) {
+        const float x = -ld_plain(row + e.at), t = fmaxf(top, x);
+        total = fmaf(total, expf(top - t), expf(x - t));
+        top = t;
+      }
+    }
+    const float t = lanes_max<W>(top);
+    total = lanes_sum<W>(total * expf(top - t));
+    top = t;
+  }
+  const float held_top = top;                  // what the held values are relative to
+  if (G == T) {
+    if (lane == 0) stats[tid >> 5] = make_float2(top, total);
+    __syncthreads();
+    const float2 p = lane < T / 32 ? stats[lane] : make_float2(-FLT_MAX, 0.f);
+    top = lanes_max<32>(p.x);
+    total = lanes_sum<32>(p.y * expf(p.x - top));
+    if (tid == 0) factors[0] = row_numbers<POLICY, 1>(z, labels, mine, true, J, make_float2(top, total), out, pol);
     if (!POLICY) return;
     __syncthreads();
-    f = factor;
   } else {
-    f = row_numbers(r, live, z_label, make_float2(top, total), out, pol, POLICY, ok && gl == 0);
-  }
-  if (!POLICY || pol.dz == nullptr || !ok) return;
-  const float scale = f * (exp_term(mine - top) / total);
-#pragma unroll
-  for (int k = 0; k < 4 * NV; ++k) v.x[k] = f == 0.f ? 0.f : v.x[k] * scale;
-  store_row<NV>(pol.dz + r * J, row, v, J, label, f, first, G);
-}
-
-// Rows longer than a cluster's registers: a CTA of T threads per row goes through it once for the sums, by element, and once more for
-// the gradient.
-template <int T, bool POLICY>
-__global__ void __launch_bounds__(T)
-choice_long_rows_kernel(const float* z, const long long* labels, RowOut out, Policy pol, long long R, int J) {
-  chain_wait();
-  chain_next();
-  __shared__ float2 part[32];
-  __shared__ float factor;
-  const long long r = blockIdx.x;
-  const long long label = ld_plain(labels + r);
-  const bool live = counts(label, J);
-  const float* row = z + r * J;
-  float top = -FLT_MAX, total = 0.f;
-  if (live)
-    for (int j0 = threadIdx.x; j0 < J; j0 += 4 * T) {
-      float x[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) x[c] = j0 + c * T < J ? -ld_plain(row + j0 + c * T) : -CUDART_INF_F;
-      const float t = fmaxf(fmaxf(top, fmaxf(x[0], x[1])), fmaxf(x[2], x[3]));
-      total = total * exp_term(top - t) + ((exp_term(x[0] - t) + exp_term(x[1] - t)) + (exp_term(x[2] - t) + exp_term(x[3] - t)));
-      top = t;
+    if (gl == 0) stats[own] = make_float2(top, total);
+    if (T > 32) __syncthreads(); else __syncwarp();
+    if (kRows > 32 || tid < 32) {
+      const float f = row_numbers<POLICY, kRows>(z, labels, mine, mine_ok, J, stats[tid < kRows ? tid : 0], out, pol);
+      if (tid < kRows) factors[tid] = f;
     }
-  float t = lanes_max<32>(top);
-  total = lanes_sum<32>(total * exp_term(top - t));
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_float2(t, total);
-  __syncthreads();
-  const int lane = threadIdx.x & 31;
-  const float2 p = lane < T / 32 ? part[lane] : make_float2(-FLT_MAX, 0.f);
-  top = lanes_max<32>(p.x);
-  total = lanes_sum<32>(p.y * exp_term(p.x - top));
-  if (threadIdx.x == 0) factor = row_numbers(r, live, live ? ld_plain(row + label) : 0.f, make_float2(top, total), out, pol, POLICY, true);
-  if (!POLICY || pol.dz == nullptr) return;
-  __syncthreads();
-  const float f = factor, scale = f / total;
-  float* to = pol.dz + r * J;
-  for (int j = threadIdx.x; j < J; j += T)
-    to[j] = f == 0.f ? 0.f : exp_term(-ld_plain(row + j) - top) * scale - (j == label ? f : 0.f);
+    if (!POLICY) return;
+    if (T > 32) __syncthreads(); else __syncwarp();
+  }
+  if (pol.dz == nullptr || !ok) return;
+  const float f = factors[own];
+  if constexpr (HOLD) {
+    float* to = pol.dz + r * J;
+    const float scale = f * (expf(held_top - top) / total);
+#pragma unroll
+    for (int k = 0; k < 4 * NV; ++k) v.x[k] = f == 0.f ? 0.f : v.x[k] * scale;
+    store_row<NV>(to, row, v, J, label, f, gl, G);
+  } else {
+    grad_row<(T < 1024 ? 2 : NV)>(row, (char*)pol.dz - (char*)z, e, 0, e.vectors, gl, G, top, f == 0.f ? 0.f : f / total, f, (int)label);
+  }
 }
 
 // dz = factor * (p - onehot), from the kept (top, total): no sums, so a row is cut into chunks of a CTA where it is long. From the last
 // row to the first: the forward has gone the other way, and what it read last may still be in L2.
-template <int T, int G, int NV>
+template <int T, int G, int NV, bool HOLD>
 __global__ void __launch_bounds__(T)
 choice_grad_kernel(const float* z, const long long* labels, const float2* stats, const float* factor, const float* gout,
                    float* __restrict__ dz, long long R, int J, int chunks) {
@@ -362,16 +482,23 @@ choice_grad_kernel(const float* z, const long long* labels, const float2* stats,
   const long long back = G == T ? (long long)(blockIdx.x / chunks) : (long long)blockIdx.x * (T / G) + threadIdx.x / G;
   if (back >= R) return;
   const long long r = R - 1 - back;
-  const int first = (G == T ? (int)(blockIdx.x % chunks) * G * NV : 0) + gl;
   const long long label = ld_plain(labels + r);
-  const float f = ld_plain(factor + r) * (gout ? ld_plain(gout) : 1.f);
-  const bool live = counts(label, J) && f != 0.f;
+  float f = ld_plain(factor + r) * (gout ? ld_plain(gout) : 1.f);
+  if (!counts(label, J)) f = 0.f;
   const float2 st = ld_plain(stats + r);
-  RowValues<NV> v = load_row<NV>(z + r * J, J, live, first, G);
-  const float scale = live ? f / st.y : 0.f;
+  const float scale = f == 0.f ? 0.f : f / st.y;
+  const float* row = z + r * J;
+  if constexpr (HOLD) {
+    float* to = dz + r * J;
+    const int first = G == T ? (int)(blockIdx.x % chunks) * G * NV + gl : gl;
+    RowValues<NV> v = load_row<NV>(row, J, f != 0.f, first, G);
 #pragma unroll
-  for (int k = 0; k < 4 * NV; ++k) v.x[k] = live ? exp_term(v.x[k] - st.x) * scale : 0.f;
-  store_row<NV>(dz + r * J, z + r * J, v, J, label, live ? f : 0.f, first, G);
+    for (int k = 0; k < 4 * NV; ++k) v.x[k] = f == 0.f ? 0.f : exp_term(v.x[k] - st.x) * scale;
+    store_row<NV>(to, row, v, J, label, f, first, G);
+  } else {
+    const Ends e(row, J, gl);
+    grad_row<NV>(row, (char*)dz - (char*)z, e, 0, e.vectors, gl, G, st.x, scale, f, (int)label);
+  }
 }
 
 // dz *= *gout, unless that is 1 (the loss is the whole objective): then there is nothing to do
@@ -454,46 +581,52 @@ struct RowShape {
   bool fits(int lanes, int nv) const { return J + slack <= 4 * lanes * nv; }
 };
 
-template <int T, int G, int NV, bool POLICY>
-int launch_rows_as(unsigned cluster, const float* z, const long long* labels, const RowOut& out, const Policy& pol, long long R, int J,
-                   cudaStream_t s) {
-  if constexpr (G == T) {
-    if (cluster > 1) {
-      (void)launch_chained(choice_rows_kernel<T, G, NV, true, POLICY>, (unsigned)R * cluster, T, 0, s, cluster, z, labels, out, pol, R, J);
-      return done();
-    }
-  }
-  const unsigned grid = G == T ? (unsigned)R : (unsigned)((R + T / G - 1) / (T / G));
-  (void)launch_chained(choice_rows_kernel<T, G, NV, false, POLICY>, grid, T, 0, s, 0, z, labels, out, pol, R, J);
-  return done();
+template <int T_, int G_, int NV_, bool HOLD_>
+struct Lanes {
+  static constexpr int T = T_, G = G_, NV = NV_;
+  static constexpr bool HOLD = HOLD_;
+};
+// Calls as() with the kernel's shape for rows of this length: the fewest lanes that hold one in eight vectors each, as every lane less shares the
+// row's numbers and shuffles among more rows (131 072 rows of 125: 37 us with a warp each, 14.6 with four lanes); beyond a warp's 1024
+// elements a warp that streams, then a CTA as large as leaves a lane some 32 elements: what follows a row's last load -- joins, its
+// numbers -- takes a CTA's time whatever its size (16 384 rows of 3001, with gradient: T = 128 85 us, 512 152; 8192 of 50 021: 779, 573
+// with 1024).
+template <typename As>
+auto by_length(const RowShape& w, int warp_row, As as) {
+  if (w.fits(1, 4)) return as(Lanes<256, 1, 4, true>{});
+  if (w.fits(1, 8)) return as(Lanes<256, 1, 8, true>{});
+  if (w.fits(2, 8)) return as(Lanes<256, 2, 8, true>{});
+  if (w.fits(4, 8)) return as(Lanes<256, 4, 8, true>{});
+  if (w.fits(8, 8)) return as(Lanes<256, 8, 8, true>{});
+  if (w.fits(16, 8)) return as(Lanes<256, 16, 8, true>{});
+  if (w.fits(32, 8)) return as(Lanes<256, 32, 8, true>{});
+  if (w.J <= warp_row) return as(Lanes<256, 32, 4, false>{});
+  if (w.J <= 6000) return as(Lanes<128, 128, 4, false>{});
+  if (w.J <= 12000) return as(Lanes<256, 256, 4, false>{});
+  if (w.J <= 24000) return as(Lanes<512, 512, 4, false>{});
+  return as(Lanes<1024, 1024, 4, false>{});
 }
 
 template <bool POLICY>
-int launch_rows(const float* z, const long long* labels, const RowOut& out, const Policy& pol, long long R, int J, cudaStream_t s) {
-  const RowShape w(z, J);
-  if (w.fits(4, 1)) return launch_rows_as<256, 4, 1, POLICY>(1, z, labels, out, pol, R, J, s);
-  if (w.fits(8, 1)) return launch_rows_as<256, 8, 1, POLICY>(1, z, labels, out, pol, R, J, s);
-  if (w.fits(16, 1)) return launch_rows_as<256, 16, 1, POLICY>(1, z, labels, out, pol, R, J, s);
-  if (w.fits(32, 1)) return launch_rows_as<256, 32, 1, POLICY>(1, z, labels, out, pol, R, J, s);
-  if (w.fits(32, 2)) return launch_rows_as<256, 32, 2, POLICY>(1, z, labels, out, pol, R, J, s);
-  if (w.fits(32, 4)) return launch_rows_as<256, 32, 4, POLICY>(1, z, labels, out, pol, R, J, s);
-  if (w.fits(32, 8)) return launch_rows_as<256, 32, 8, POLICY>(1, z, labels, out, pol, R, J, s);
-  if (w.fits(128, 4)) return launch_rows_as<128, 128, 4, POLICY>(1, z, labels, out, pol, R, J, s);
-  if (w.fits(256, 4)) return launch_rows_as<256, 256, 4, POLICY>(1, z, labels, out, pol, R, J, s);
-  if (w.fits(256, 8)) return launch_rows_as<256, 256, 8, POLICY>(1, z, labels, out, pol, R, J, s);
-  for (unsigned cluster = 1; cluster <= 8; cluster *= 2)
-    if (w.fits(512 * (int)cluster, 8)) return launch_rows_as<512, 512, 8, POLICY>(cluster, z, labels, out, pol, R, J, s);
-  (void)launch_chained(choice_long_rows_kernel<512, POLICY>, (unsigned)R, 512, 0, s, 0, z, labels, out, pol, R, J);
-  return done();
+int launch_rows(const float* z, const long long* labels, const RowOut& out, const Policy& pol, long long R, int J, cudaStream_t s,
+                unsigned* ctas = nullptr) {
+  return by_length(RowShape(z, J), POLICY ? 1800 : 6000, [&](auto lanes) {
+    using L = decltype(lanes);
+    constexpr int T = L::T, G = L::G;
+    const unsigned grid = (unsigned)((R + T / G - 1) / (T / G));
+    if (ctas) *ctas = grid;
+    (void)launch_chained(choice_rows_kernel<T, G, L::NV, L::HOLD, POLICY>, grid, T, 0, s, 0, z, labels, out, pol, R, J);
+    return done();
+  });
 }
 
-template <int T, int G, int NV>
+template <int T, int G, int NV, bool HOLD>
 int launch_grad_as(const float* z, const long long* labels, const float* stats, const float* factor, const float* gout, float* dz,
                    long long R, int J, cudaStream_t s) {
-  const int chunks = G == T ? (int)(((long long)J + 3 + 4 * T * NV - 1) / (4 * T * NV)) : 1;
+  const int chunks = G == T ? (J + 3 + 4 * T * NV - 1) / (4 * T * NV) : 1;   // (up to three elements of the first vector are the row in front's)
   const long long grid = G == T ? R * chunks : (R + T / G - 1) / (T / G);
   if (grid > 0x7fffffffLL) return SNNTC_E_TOO_LARGE;
-  (void)launch_chained(choice_grad_kernel<T, G, NV>, (unsigned)grid, T, 0, s, 0, z, labels, (const float2*)stats, factor, gout, dz, R, J, chunks);
+  (void)launch_chained(choice_grad_kernel<T, G, NV, HOLD>, (unsigned)grid, T, 0, s, 0, z, labels, (const float2*)stats, factor, gout, dz, R, J, chunks);
   return done();
 }
 
@@ -515,12 +648,11 @@ int snntc_choice_backward(const float* z, const long long* labels, const float* 
   if (!z || !labels || !stats_2R || !factor || !dz) return SNNTC_E_NULL;
   if (const int rc = check_rows(R, J)) return rc;
   cudaStream_t s = (cudaStream_t)stream;
-  const RowShape w(z, J);
-  if (w.fits(4, 1)) return launch_grad_as<256, 4, 1>(z, labels, stats_2R, factor, gout, dz, R, J, s);
-  if (w.fits(16, 1)) return launch_grad_as<256, 16, 1>(z, labels, stats_2R, factor, gout, dz, R, J, s);
-  if (w.fits(32, 2)) return launch_grad_as<256, 32, 2>(z, labels, stats_2R, factor, gout, dz, R, J, s);
-  if (w.fits(32, 4)) return launch_grad_as<256, 32, 4>(z, labels, stats_2R, factor, gout, dz, R, J, s);
-  return launch_grad_as<256, 256, 4>(z, labels, stats_2R, factor, gout, dz, R, J, s);
+  return by_length(RowShape(z, J), 1800, [&](auto lanes) {
+    using L = decltype(lanes);
+    if constexpr (L::G == L::T) return launch_grad_as<128, 128, 4, true>(z, labels, stats_2R, factor, gout, dz, R, J, s);
+    else return launch_grad_as<L::T, L::G, L::NV, L::HOLD>(z, labels, stats_2R, factor, gout, dz, R, J, s);
+  });
 }
 
 size_t snntc_policy_loss_workspace_bytes(long long R) { return R <= 0 ? 0 : (size_t)R * sizeof(double3) + 256; }
@@ -539,8 +671,9 @@ int snntc_policy_loss(const float* z, const long long* labels, const float* old_
   (void)launch_chained(policy_count_kernel, ctas, kSumThreads, 0, s, ctas, labels, inv_n, R, J);
   if (const int rc = done()) return rc;
   const Policy pol{old_logp, advantage, ref_logp, inv_n, terms, dz, PolicyParams{1 - clip_low, 1 + clip_high, kl_coef}};
-  if (const int rc = launch_rows<true>(z, labels, RowOut{nullptr, nullptr, (float2*)stats_2R, factor}, pol, R, J, s)) return rc;
-  (void)launch_chained(policy_mean_kernel, ctas, kSumThreads, 0, s, ctas, terms, inv_n, loss, kl_and_clipped, R);
+  unsigned n = 0;                              // CTAs, and so terms
+  if (const int rc = launch_rows<true>(z, labels, RowOut{nullptr, nullptr, (float2*)stats_2R, factor}, pol, R, J, s, &n)) return rc;
+  (void)launch_chained(policy_mean_kernel, sum_ctas(n), kSumThreads, 0, s, sum_ctas(n), terms, inv_n, loss, kl_and_clipped, (long long)n);
   return done();
 }
 
