@@ -41,6 +41,7 @@ template <> struct Vec<1> {
   static __device__ __forceinline__ Vec load(const float* p) { return {{ld_plain(p)}}; }
   static __device__ __forceinline__ Vec load_once(const float* p) { return {{__ldcs(p)}}; }
   __device__ __forceinline__ void store(float* p) const { *p = v[0]; }
+  __device__ __forceinline__ void store_once(float* p) const { __stcs(p, v[0]); }
 };
 template <> struct Vec<4> {
   float v[4];
@@ -48,46 +49,54 @@ template <> struct Vec<4> {
   static __device__ __forceinline__ Vec load(const float* p) { return of(ld_plain((const float4*)p)); }
   static __device__ __forceinline__ Vec load_once(const float* p) { return of(__ldcs((const float4*)p)); }
   __device__ __forceinline__ void store(float* p) const { *(float4*)p = make_float4(v[0], v[1], v[2], v[3]); }
+  __device__ __forceinline__ void store_once(float* p) const { __stcs((float4*)p, make_float4(v[0], v[1], v[2], v[3])); }
 };
 
 constexpr int kThreads = 256;
-constexpr int kRowsAhead = 4;
-
-// L lanes to a row of `vectors` vectors, kRowsAhead rows of a lane in flight: the id and then its row are two loads one behind the other.
-template <int VEC>
+// L lanes to a row of `vectors` vectors. A lane has AHEAD rows in flight -- an id and then its row are two loads one behind the other -- and
+// of each COLUMNS vectors, so that what a row's read opens in memory is read at once. us, (AHEAD, COLUMNS) = (4, 1), (2, 2), (1, 4): 131 072
+// rows of 512 values 65.6, 59.6, 61.7; 10^6 of 64 67.8, 92, 123 (one vector a lane: the second is never there).
+template <int VEC, int AHEAD, int COLUMNS>
 __global__ void __launch_bounds__(kThreads)
 embed_forward_kernel(Ids ids, const float* table, float* __restrict__ y, long long N, int D, int vectors, int L, float scale, int spikes,
                      float no_spike) {
   chain_wait();
   chain_next();
   const int rows = kThreads / L, gl = threadIdx.x % L;
-  const long long t0 = (long long)blockIdx.x * rows * kRowsAhead + threadIdx.x / L;
-  unsigned key[kRowsAhead];
+  const long long t0 = (long long)blockIdx.x * rows * AHEAD + threadIdx.x / L;
+  unsigned key[AHEAD];
 #pragma unroll
-  for (int k = 0; k < kRowsAhead; ++k) key[k] = t0 + k * rows < N ? key_of(ids, t0 + k * rows) : (unsigned)ids.V;
-  for (int c = gl; c < vectors; c += L) {
-    Vec<VEC> q[kRowsAhead];
+  for (int k = 0; k < AHEAD; ++k) key[k] = t0 + k * rows < N ? key_of(ids, t0 + k * rows) : (unsigned)ids.V;
+  for (int c0 = gl; c0 < vectors; c0 += COLUMNS * L) {
+    Vec<VEC> q[AHEAD][COLUMNS];
 #pragma unroll
-    for (int k = 0; k < kRowsAhead; ++k)
-      if (key[k] != (unsigned)ids.V) q[k] = Vec<VEC>::load(table + (long long)key[k] * D + c * VEC);
+    for (int k = 0; k < AHEAD; ++k)
 #pragma unroll
-    for (int k = 0; k < kRowsAhead; ++k) {
+      for (int m = 0; m < COLUMNS; ++m)
+        if (key[k] != (unsigned)ids.V && c0 + m * L < vectors) q[k][m] = Vec<VEC>::load(table + (long long)key[k] * D + (c0 + m * L) * VEC);
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
       if (t0 + k * rows >= N) break;
       const bool token = key[k] != (unsigned)ids.V;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) q[k].v[j] = token ? value_of(q[k].v[j], scale, spikes) : no_spike;
-      q[k].store(y + (t0 + k * rows) * D + c * VEC);
+      for (int m = 0; m < COLUMNS; ++m) {
+        if (c0 + m * L >= vectors) break;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) q[k][m].v[j] = token ? value_of(q[k][m].v[j], scale, spikes) : no_spike;
+        q[k][m].store_once(y + (t0 + k * rows) * D + (c0 + m * L) * VEC);
+      }
     }
   }
 }
 
-// ---- sort. Up to kSmallSort pairs by one CTA in shared memory. More: tiles of consecutive keys, one CTA each; a pass is the count of every
-// digit in every tile, then the scatter, whose CTAs add up the counts in front of their own.
-constexpr int kSmallSort = 4096;
+// ---- sort. Up to kSmallSort pairs: every pair's place is the number of pairs in front of it, counted by comparison with all. More: tiles
+// of consecutive keys, one CTA each; a pass is the count of every digit in every tile, then the scatter, whose CTAs add up the counts in
+// front of their own.
+constexpr int kSmallSort = 8192;
 constexpr int kSortThreads = 512;
 constexpr int kDigits = 512;              // of nine bits
 constexpr int kTiles = 148;
-constexpr int kTileKeys = 2048;           // at least
+constexpr int kTileKeys = 2048;           // of a tile at a time
 
 struct Keys {                 // the first pass reads the ids, the later ones pairs
   Ids ids;
@@ -97,23 +106,42 @@ __device__ __forceinline__ uint2 pair_at(const Keys& k, long long t) {
   return k.pairs ? ld_plain(k.pairs + t) : make_uint2(key_of(k.ids, t), (unsigned)t);
 }
 
-// A bitonic network over (key << 32 | position): keys in order, equal ones by position.
-__global__ void __launch_bounds__(1024) sort_small_kernel(Ids ids, uint2* __restrict__ out, int N, int size) {
+// 32 pairs to a CTA, a lane each; a warp counts in its eighth of the keys, four to a load that all lanes share. N^2 comparisons: 4096 pairs
+// are 1 us of them. An equal key counts where its position is lower.
+__global__ void __launch_bounds__(kThreads) sort_small_kernel(Ids ids, uint2* __restrict__ out, int N) {
   chain_wait();
   chain_next();
-  __shared__ unsigned long long s[kSmallSort];
-  for (int t = threadIdx.x; t < size; t += 1024) s[t] = t < N ? (unsigned long long)key_of(ids, t) << 32 | (unsigned)t : ~0ull;
-  for (int k = 2; k <= size; k <<= 1)
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < size / 2; i += 1024) {
-        const int a = 2 * i - (i & (j - 1)), b = a + j;
-        const unsigned long long x = s[a], y = s[b];
-        if ((x > y) == ((a & k) == 0)) { s[a] = y; s[b] = x; }
-      }
-    }
+  constexpr int kWarps = kThreads / 32;
+  __shared__ __align__(16) unsigned keys[kSmallSort];
+  __shared__ int counted[kWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i0 = blockIdx.x * 32, i = i0 + lane;
+  const unsigned key = i < N ? key_of(ids, i) : 0;
+  const int share = ((N + kWarps - 1) / kWarps + 3) / 4 * 4, j0 = warp * share, j1 = min(N, j0 + share), end = j0 < N ? (j1 + 3) / 4 * 4 : j0;
+#pragma unroll 8
+  for (int j = j0 + lane; j < end; j += 32) keys[j] = j < j1 ? key_of(ids, j) : 0xffffffffu;
+  __syncwarp();
+  int n = 0;
+  // keys in front of the CTA's own, its own, and those behind (i0 and the shares are multiples of four)
+  const int own0 = min(max(i0, j0), end), own1 = min(max(i0 + 32, j0), end);
+#pragma unroll 8
+  for (int j = j0; j < own0; j += 4) {
+    const uint4 q = *(const uint4*)&keys[j];
+    n += (q.x <= key) + (q.y <= key) + (q.z <= key) + (q.w <= key);
+  }
+  for (int j = own0; j < own1; ++j) n += keys[j] < key || (keys[j] == key && j < i);
+#pragma unroll 8
+  for (int j = own1; j < end; j += 4) {
+    const uint4 q = *(const uint4*)&keys[j];
+    n += (q.x < key) + (q.y < key) + (q.z < key) + (q.w < key);
+  }
+  counted[warp][lane] = n;
   __syncthreads();
-  for (int t = threadIdx.x; t < N; t += 1024) out[t] = make_uint2((unsigned)(s[t] >> 32), (unsigned)s[t]);
+  if (warp == 0 && i < N) {
+    int place = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) place += counted[w][lane];
+    out[place] = make_uint2(key, (unsigned)i);
+  }
 }
 
 __global__ void __launch_bounds__(kSortThreads)
@@ -133,11 +161,12 @@ __global__ void __launch_bounds__(kSortThreads)
 sort_scatter_kernel(Keys keys, const int* counts, uint2* __restrict__ out, long long N, long long tile, int tiles, int shift, int digits) {
   chain_wait();
   chain_next();
-  constexpr int kWarps = kSortThreads / 32;
+  constexpr int kWarps = kSortThreads / 32, kEach = kTileKeys / kSortThreads, kOfWarp = 32 * kEach;
   __shared__ int next[kDigits];             // where the next key of a digit goes
-  __shared__ int of_warp[kWarps][kDigits];  // keys of a digit in a warp's 32, then those of the warps in front
+  __shared__ int of_warp[kWarps][kDigits];  // keys of a digit in a warp's stretch, then those of the warps in front
   __shared__ int warp_sum[kWarps];
   const int d = threadIdx.x, lane = d & 31, warp = d >> 5;
+  const long long t0 = blockIdx.x * tile, t1 = min(N, t0 + tile);
   int before = 0, total = 0;
 #pragma unroll 16
   for (int k = 0; k < tiles; ++k) {
@@ -157,14 +186,28 @@ sort_scatter_kernel(Keys keys, const int* counts, uint2* __restrict__ out, long 
   __syncthreads();
   for (int w = 0; w < warp; ++w) upto += warp_sum[w];
   next[d] = upto - total + before;
-  const long long t0 = blockIdx.x * tile, t1 = min(N, t0 + tile);
-  for (long long t = t0; t < t1; t += kSortThreads) {
-    const bool ok = t + d < t1;
-    const uint2 p = ok ? pair_at(keys, t + d) : make_uint2(0, 0);
-    const unsigned digit = ok ? (p.x >> shift) & (digits - 1) : kDigits;
-    const unsigned same = __match_any_sync(0xffffffffu, digit);
-    const int rank = __popc(same & ((1u << lane) - 1));
-    if (ok && rank == 0) of_warp[warp][digit] = __popc(same);
+  for (long long t = t0; t < t1; t += kTileKeys) {
+    // every warp ranks a stretch of its own, 32 keys at a time, against the counts of its earlier ones
+    uint2 p[kEach];
+    int digit[kEach], rank[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const long long at = t + warp * kOfWarp + k * 32 + lane;
+      digit[k] = -1;
+      if (at < t1) {
+        p[k] = pair_at(keys, at);
+        digit[k] = (int)((p[k].x >> shift) & (digits - 1));
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const unsigned same = __match_any_sync(0xffffffffu, digit[k]);
+      const int in_front = digit[k] >= 0 ? of_warp[warp][digit[k]] : 0;
+      rank[k] = in_front + __popc(same & ((1u << lane) - 1));
+      __syncwarp();
+      if (digit[k] >= 0 && (same >> lane) == 1) of_warp[warp][digit[k]] = rank[k] + 1;    // the last lane of its digit
+      __syncwarp();
+    }
     __syncthreads();
     int sum = 0;
 #pragma unroll
@@ -174,7 +217,10 @@ sort_scatter_kernel(Keys keys, const int* counts, uint2* __restrict__ out, long 
       sum += c;
     }
     __syncthreads();
-    if (ok) out[next[digit] + of_warp[warp][digit] + rank] = p;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k)
+      if (digit[k] >= 0) out[next[digit[k]] + of_warp[warp][digit[k]] + rank[k]] = p[k];
+    if (t + kTileKeys >= t1) break;
     __syncthreads();
     next[d] += sum;
 #pragma unroll
@@ -187,16 +233,17 @@ sort_scatter_kernel(Keys keys, const int* counts, uint2* __restrict__ out, long 
 // kTermsAhead rows of g in flight. Runs inside a tile are done there and then; of one that crosses a border the first tile leaves its
 // part in `tail`, the others theirs in `head`, and the joining kernel adds those in order. So a token that every second place holds is
 // summed by as many CTAs as its share, and the order of summation depends on the sizes alone.
-// Rows that no token names are zeroed by further CTAs of the same launch, a warp for 32 rows: each lane looks its row up in the sorted keys.
+// Rows that no token names are zeroed by further CTAs of the same launch, a warp for 32 rows or a share of them: each lane looks
+// a row up in the sorted keys.
 constexpr int kTermsAhead = 8;
-constexpr int kSumTiles = 2048;           // at most
+constexpr int kSumTiles = 2048;           // at most, of rows that take a warp
 
 struct RunSums {
   const uint2* pairs;
   const float *g, *table;
   float *dtable, *head, *tail;            // parts: [tiles][D]
   long long N, V;
-  int D, vectors, L, slices, M, tiles, sum_ctas;
+  int D, vectors, L, slices, M, tiles, sum_ctas, zero_shares;
   float scale;
   int spikes;
 };
@@ -215,29 +262,39 @@ __device__ __forceinline__ void write_row(const RunSums& q, unsigned key, int c,
   sum.store(q.dtable + at);
 }
 
-template <int VEC>
 __device__ void zero_rows(const RunSums& q) {
   const int lane = threadIdx.x & 31;
-  const long long v0 = ((long long)(blockIdx.x - q.sum_ctas) * (kThreads / 32) + (threadIdx.x >> 5)) * 32;
+  const long long unit = (long long)(blockIdx.x - q.sum_ctas) * (kThreads / 32) + (threadIdx.x >> 5), v0 = unit / q.zero_shares * 32;
+  const int share = (int)(unit % q.zero_shares);
   if (v0 >= q.V) return;
-  long long lo = 0, hi = q.N;             // the first place whose key is not below the lane's row
+  // the places [lo, hi) whose keys are of these 32 rows, by 32 probes at a time for each end; then every lane looks for its own in there
+  long long lo = 0, hi = 0, step = (q.N + 33) / 33;
+  for (long long left = q.N; left > 0; left = step - 1, step = (left + 33) / 33) {
+    const long long a = lo + (lane + 1) * step - 1, b = hi + (lane + 1) * step - 1;
+    const bool below = a < min(q.N, lo + left) && ld_plain(&q.pairs[a].x) < v0, under = b < min(q.N, hi + left) && ld_plain(&q.pairs[b].x) < v0 + 32;
+    lo += __popc(__ballot_sync(0xffffffffu, below)) * step;
+    hi += __popc(__ballot_sync(0xffffffffu, under)) * step;
+  }
+  const long long end = hi;
   while (lo < hi) {
     const long long mid = (lo + hi) >> 1;
     if (ld_plain(&q.pairs[mid].x) < v0 + lane) lo = mid + 1;
     else hi = mid;
   }
-  const bool empty = v0 + lane < q.V && !(lo < q.N && ld_plain(&q.pairs[lo].x) == v0 + lane);
-  const unsigned todo = __ballot_sync(0xffffffffu, empty);
-  const Vec<VEC> zero = {};
-  if (q.vectors >= 32) {
-    for (unsigned m = todo; m; m &= m - 1) {
-      float* row = q.dtable + (v0 + __ffs(m) - 1) * q.D;
-      for (int c = lane; c < q.vectors; c += 32) zero.store(row + c * VEC);
+  const bool empty = v0 + lane < q.V && !(lo < end && ld_plain(&q.pairs[lo].x) == v0 + lane);
+  unsigned todo = __ballot_sync(0xffffffffu, empty);
+  while (todo) {                          // rows behind one another are one stretch of floats; this warp's share of it, in whole vectors
+    const int first = __ffs(todo) - 1, rows = __ffs(~(todo >> first)) - 1 < 0 ? 32 - first : __ffs(~(todo >> first)) - 1;
+    todo &= rows == 32 ? 0u : ~(((1u << rows) - 1) << first);
+    float* at = q.dtable + (v0 + first) * q.D;
+    const long long n = (long long)rows * q.D;
+    const long long head = min(n, (long long)((4 - ((uintptr_t)at >> 2)) & 3)), vectors = (n - head) / 4, tail = head + 4 * vectors;
+    const long long each = (vectors + q.zero_shares - 1) / q.zero_shares, a = share * each, b = min(vectors, a + each);
+    for (long long k = a + lane; k < b; k += 32) __stcs((float4*)(at + head) + k, make_float4(0.f, 0.f, 0.f, 0.f));
+    if (share == 0) {
+      if (lane < head) at[lane] = 0.f;
+      if (lane < n - tail) at[tail + lane] = 0.f;
     }
-  } else if (todo) {                      // short rows: the 32 of them are one stretch
-    float* rows = q.dtable + v0 * q.D;
-    for (int e = lane; e < 32 * q.vectors; e += 32)
-      if (todo >> (e / q.vectors) & 1) zero.store(rows + e * VEC);
   }
 }
 
@@ -245,7 +302,7 @@ template <int VEC>
 __global__ void __launch_bounds__(kThreads) embed_run_sums_kernel(RunSums q) {
   chain_wait();
   chain_next();
-  if ((int)blockIdx.x >= q.sum_ctas) return zero_rows<VEC>(q);
+  if ((int)blockIdx.x >= q.sum_ctas) return zero_rows(q);
   const long long unit = ((long long)blockIdx.x * kThreads + threadIdx.x) / q.L;
   const int tile = (int)(unit / q.slices), c = (int)(unit % q.slices) * q.L + threadIdx.x % q.L;
   if (tile >= q.tiles || c >= q.vectors) return;
@@ -283,42 +340,63 @@ __global__ void __launch_bounds__(kThreads) embed_run_sums_kernel(RunSums q) {
   else write_row<VEC>(q, key, c, sum);
 }
 
-// One CTA per tile; it has work where a run begins in the tile and goes on behind it.
+// Runs that go on behind the tile in which they begin: a warp looks at a tile and 32 vectors, adds a run of a few tiles itself and leaves
+// a longer one to all warps of its CTA, an eighth of the tiles each.
 template <int VEC>
 __global__ void __launch_bounds__(kThreads) embed_join_kernel(RunSums q) {
   chain_wait();
   chain_next();
-  constexpr int kWarps = kThreads / 32;
+  constexpr int kWarps = kThreads / 32, kFew = 8;
   __shared__ Vec<VEC> part[kWarps][32];
-  const int tile = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long i0 = (long long)tile * q.M, i1 = i0 + q.M;
-  if (i1 >= q.N) return;
-  const unsigned key = ld_plain(&q.pairs[i1 - 1].x);
-  if (key >= q.V || ld_plain(&q.pairs[i1].x) != key || (i0 > 0 && ld_plain(&q.pairs[i0 - 1].x) == key)) return;
-  int lo = tile + 1, hi = q.tiles - 1;     // the last tile that begins with this key
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (ld_plain(&q.pairs[(long long)mid * q.M].x) == key) lo = mid;
-    else hi = mid - 1;
+  __shared__ int last_tile[kWarps];        // of a run that is left to all; 0: none (a run's last tile is behind its first)
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.y * 32 + lane;
+  const auto head_of = [&](int t) { return Vec<VEC>::load(q.head + (long long)t * q.D + c * VEC); };
+  const auto add = [](Vec<VEC>& sum, const Vec<VEC>& x) {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) sum.v[j] += x.v[j];
+  };
+  {
+    const int tile = blockIdx.x * kWarps + warp;
+    const long long i0 = (long long)tile * q.M, i1 = i0 + q.M;
+    int last = 0;
+    unsigned key = 0;
+    if (i1 < q.N) {
+      key = ld_plain(&q.pairs[i1 - 1].x);
+      const unsigned after = ld_plain(&q.pairs[i1].x), before = i0 > 0 ? ld_plain(&q.pairs[i0 - 1].x) : 0xffffffffu;
+      if (key < q.V && after == key && before != key) {
+        last = tile + 1;                   // the last tile that begins with this key, by 32 probes at a time
+        for (int left = q.tiles - 1 - last, step = (left + 33) / 33; left > 0; left = step - 1, step = (left + 33) / 33) {
+          const int t = last + (lane + 1) * step;
+          const bool same = t <= last + left && t < q.tiles && ld_plain(&q.pairs[(long long)t * q.M].x) == key;
+          last += __popc(__ballot_sync(0xffffffffu, same)) * step;
+        }
+      }
+    }
+    if (last && last - tile <= kFew) {
+      if (c < q.vectors) {
+        Vec<VEC> sum = Vec<VEC>::load(q.tail + (long long)tile * q.D + c * VEC);
+#pragma unroll 4
+        for (int t = tile + 1; t <= last; ++t) add(sum, head_of(t));
+        write_row<VEC>(q, key, c, sum);
+      }
+      last = 0;
+    }
+    if (lane == 0) last_tile[warp] = last;
   }
-  for (int c0 = 0; c0 < q.vectors; c0 += 32) {
-    const int c = c0 + lane;
+  __syncthreads();
+  for (int k = 0; k < kWarps; ++k) {
+    const int last = last_tile[k], tile = blockIdx.x * kWarps + k;
+    if (last == 0) continue;
     Vec<VEC> sum = {};
     if (c < q.vectors)
 #pragma unroll 8
-      for (int t = tile + 1 + warp; t <= lo; t += kWarps) {
-        const Vec<VEC> x = Vec<VEC>::load(q.head + (long long)t * q.D + c * VEC);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sum.v[j] += x.v[j];
-      }
+      for (int t = tile + 1 + warp; t <= last; t += kWarps) add(sum, head_of(t));
     part[warp][lane] = sum;
     __syncthreads();
     if (warp == 0 && c < q.vectors) {
       sum = Vec<VEC>::load(q.tail + (long long)tile * q.D + c * VEC);
-      for (int w = 0; w < kWarps; ++w)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sum.v[j] += part[w][lane].v[j];
-      write_row<VEC>(q, key, c, sum);
+      for (int w = 0; w < kWarps; ++w) add(sum, part[w][lane]);
+      write_row<VEC>(q, ld_plain(&q.pairs[(long long)tile * q.M + q.M - 1].x), c, sum);
     }
     __syncthreads();
   }
@@ -353,16 +431,17 @@ SortPlan sort_plan(long long N, long long V) {
   p.passes = (bits + 8) / 9;
   p.bits = (bits + p.passes - 1) / p.passes;
   p.tile = (N + kTiles - 1) / kTiles;
-  if (p.tile < kTileKeys) p.tile = kTileKeys;
-  p.tile = (p.tile + kSortThreads - 1) / kSortThreads * kSortThreads;
+  p.tile = (p.tile + kTileKeys - 1) / kTileKeys * kTileKeys;
   p.tiles = (int)((N + p.tile - 1) / p.tile);
   return p;
 }
 
-// Places per tile of the sums: 32, or as many as make kSumTiles tiles
-int sum_tile(long long N) {
-  const long long m = (N + kSumTiles - 1) / kSumTiles;
-  return (int)(m < 32 ? 32 : (m + 7) / 8 * 8);
+// Places per tile of the sums: eight, one round of loads, or as many as make kSumTiles tiles; narrow rows, a few lanes each, take more tiles
+int sum_tile(long long N, int D) {
+  int lanes = 1;
+  while (lanes < 32 && lanes < (D % 4 == 0 ? D / 4 : D)) lanes *= 2;
+  const long long tiles = (long long)kSumTiles * (lanes < 4 ? 8 : 32 / lanes), m = (N + tiles - 1) / tiles;
+  return (int)((m + kTermsAhead - 1) / kTermsAhead * kTermsAhead);
 }
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
@@ -370,7 +449,7 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 struct BackwardSpace {
   size_t pairs[2], counts, head, tail, bytes;
   BackwardSpace(long long N, int D) {
-    const size_t tiles = (size_t)((N + sum_tile(N) - 1) / sum_tile(N)), parts = round256(tiles * D * sizeof(float));
+    const size_t tiles = (size_t)((N + sum_tile(N, D) - 1) / sum_tile(N, D)), parts = round256(tiles * D * sizeof(float));
     pairs[0] = 0;
     pairs[1] = round256((size_t)N * sizeof(uint2));
     counts = 2 * pairs[1];
@@ -387,11 +466,13 @@ int launch_sums(RunSums q, cudaStream_t s) {
   while (q.L < 32 && q.L < q.vectors) q.L *= 2;
   q.slices = (q.vectors + q.L - 1) / q.L;
   q.sum_ctas = (int)(((long long)q.tiles * q.slices * q.L + kThreads - 1) / kThreads);
-  const long long zero_ctas = (q.V + kThreads - 1) / kThreads;
+  // a warp zeroes up to 32 KB: 32 rows, or a share of them
+  q.zero_shares = (q.D + 255) / 256;
+  const long long zero_ctas = ((q.V + 31) / 32 * q.zero_shares + kThreads / 32 - 1) / (kThreads / 32);
   (void)launch_chained(embed_run_sums_kernel<VEC>, (unsigned)(q.sum_ctas + zero_ctas), kThreads, 0, s, 0, q);
   if (const int rc = done()) return rc;
   if (q.tiles == 1) return SNNTC_OK;
-  (void)launch_chained(embed_join_kernel<VEC>, (unsigned)q.tiles, kThreads, 0, s, 0, q);
+  (void)launch_chained(embed_join_kernel<VEC>, dim3((q.tiles + 7) / 8, (q.vectors + 31) / 32), kThreads, 0, s, 0, q);
   return done();
 }
 
@@ -406,16 +487,17 @@ int snntc_embedding_forward(const void* ids, int id_bytes, const float* table, f
   if (!ids || !table || !y) return SNNTC_E_NULL;
   const bool four = by_four(D, table, y, nullptr);
   const int vectors = four ? D / 4 : D;
-  int L = 1;                                // lanes to a row: the power of two that leaves the fewest of them idle, a warp's width at least
-  for (int l = 2; l <= kThreads; l *= 2) {
-    const auto lanes = [&](int n) { return (vectors + n - 1) / n * n; };
-    if (L < 32 ? L < vectors : lanes(l) <= lanes(L)) L = l;
-  }
-  const long long rows = (long long)kThreads / L * kRowsAhead, ctas = (N + rows - 1) / rows;
+  int L = 1;                                // lanes to a row: up to a warp
+  while (L < 32 && L < vectors) L *= 2;
   const Ids in{ids, id_bytes == 8, V, padding};
-  if (four) (void)launch_chained(embed_forward_kernel<4>, (unsigned)ctas, kThreads, 0, (cudaStream_t)stream, 0, in, table, y, N, D, vectors, L, scale, spikes, no_spike);
-  else (void)launch_chained(embed_forward_kernel<1>, (unsigned)ctas, kThreads, 0, (cudaStream_t)stream, 0, in, table, y, N, D, vectors, L, scale, spikes, no_spike);
-  return done();
+  const auto launch = [&](auto kernel, int ahead) {
+    const long long rows = (long long)kThreads / L * ahead;
+    (void)launch_chained(kernel, (unsigned)((N + rows - 1) / rows), kThreads, 0, (cudaStream_t)stream, 0, in, table, y, N, D, vectors, L,
+                         scale, spikes, no_spike);
+    return done();
+  };
+  if (vectors <= 32) return four ? launch(embed_forward_kernel<4, 4, 1>, 4) : launch(embed_forward_kernel<1, 4, 1>, 4);
+  return four ? launch(embed_forward_kernel<4, 2, 2>, 2) : launch(embed_forward_kernel<1, 2, 2>, 2);
 }
 
 size_t snntc_embedding_backward_workspace_bytes(long long N, long long V, int D) {
@@ -441,9 +523,7 @@ int snntc_embedding_backward(const void* ids, int id_bytes, const float* g, cons
   const Ids in{ids, id_bytes == 8, V, padding};
   Keys keys{in, nullptr};
   if (N <= kSmallSort) {
-    int size = 2;
-    while (size < N) size *= 2;
-    (void)launch_chained(sort_small_kernel, 1, 1024, 0, s, 0, in, pairs[0], (int)N, size);
+    (void)launch_chained(sort_small_kernel, (unsigned)((N + 31) / 32), kThreads, 0, s, 0, in, pairs[0], (int)N);
     if (const int rc = done()) return rc;
     keys.pairs = pairs[0];
   } else {
@@ -467,7 +547,7 @@ int snntc_embedding_backward(const void* ids, int id_bytes, const float* g, cons
   q.N = N;
   q.V = V;
   q.D = D;
-  q.M = sum_tile(N);
+  q.M = sum_tile(N, D);
   q.tiles = (int)((N + q.M - 1) / q.M);
   q.scale = scale;
   q.spikes = spikes;
