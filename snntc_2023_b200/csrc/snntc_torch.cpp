@@ -671,11 +671,10 @@ Tensor constant(const Tensor& t, const Tensor& like, int64_t n, const char* name
   return c;
 }
 
-Tensor choice_backward(const Tensor& z, const Tensor& label, const Tensor& stats, const Tensor& factor, const Tensor& gout, const char* what) {
+Tensor choice_backward(const Tensor& z, const Tensor& label, const float* stats, const float* factor, const Tensor& gout, const char* what) {
   const c10::cuda::CUDAGuard guard(z.device());
   const Tensor dz = empty_like_dev(z.sizes(), z);
-  check(snntc_choice_backward(ptr(z), labels_of(label), ptr(stats), ptr(factor), ptr(gout), ptr(dz), label.numel(), (int)z.size(-1), stream_of(z)),
-        what);
+  check(snntc_choice_backward(ptr(z), labels_of(label), stats, factor, ptr(gout), ptr(dz), label.numel(), (int)z.size(-1), stream_of(z)), what);
   return dz;
 }
 
@@ -698,7 +697,7 @@ struct LabelLogpFunction : torch::autograd::Function<LabelLogpFunction> {
     const auto saved = ctx->get_saved_variables();
     check_backward(saved[0], "label_log_probs");
     const Tensor g = as_cuda_f32(grads[0], "grad");
-    return {choice_backward(saved[0], saved[1], saved[2], g, Tensor(), "label_log_probs"), Tensor()};
+    return {choice_backward(saved[0], saved[1], ptr(saved[2]), ptr(g), Tensor(), "label_log_probs"), Tensor()};
   }
 };
 
@@ -715,8 +714,10 @@ struct ChoiceState : torch::CustomClassHolder {
   int P = 0;          // pairs; 0: a policy loss
   const char* name() const { return P ? "preference_loss" : "policy_loss"; }
 };
-// more: [KL term, clipped] or the margins; kept: (top, total) and the factor of every row; dz: the gradient, of a policy loss
+// more: [KL term, clipped] or the margins; dz: the gradient, of a policy loss; kept: one allocation for the workspace and, behind it, what a
+// backward reads, (top, total) and the factor of every row
 struct ChoiceLoss { Tensor loss, more, kept, dz; };
+float* kept_stats(const Tensor& kept, int64_t R) { return (float*)((char*)kept.data_ptr() + (kept.numel() - 12 * R)); }
 
 ChoiceLoss choice_loss_call(const ChoiceState& s, bool grad) {
   const Rows& r = s.rows;
@@ -724,18 +725,17 @@ ChoiceLoss choice_loss_call(const ChoiceState& s, bool grad) {
   ChoiceLoss o;
   o.loss = empty_like_dev({}, r.z);
   o.more = empty_like_dev({s.P ? s.P : 2}, r.z);
-  if (grad || s.P) o.kept = empty_like_dev({3 * r.R}, r.z);
   if (grad && !s.P) o.dz = empty_like_dev(r.z.sizes(), r.z);
-  float* stats = ptr(o.kept);
-  float* factor = stats ? stats + 2 * r.R : nullptr;
   const size_t bytes = s.P ? snntc_preference_loss_workspace_bytes(r.R, s.P) : snntc_policy_loss_workspace_bytes(r.R);
-  const Tensor ws = workspace(bytes, r.z);
+  const bool keep_rows = grad || s.P;
+  o.kept = workspace(keep_rows ? (bytes + 7) / 8 * 8 + 12 * r.R : bytes, r.z);
+  float* stats = keep_rows ? kept_stats(o.kept, r.R) : nullptr;
+  float* factor = keep_rows ? stats + 2 * r.R : nullptr;
+  void* ws = o.kept.data_ptr();
   const int rc = s.P ? snntc_preference_loss(ptr(r.z), labels_of(r.label), s.starts.defined() ? labels_of(s.starts) : nullptr, ptr(s.ref_logp),
-                                             ptr(o.loss), ptr(o.more), stats, factor, r.R, r.J, s.P, s.a, s.b, ws.data_ptr(), bytes,
-                                             stream_of(r.z))
+                                             ptr(o.loss), ptr(o.more), stats, factor, r.R, r.J, s.P, s.a, s.b, ws, bytes, stream_of(r.z))
                      : snntc_policy_loss(ptr(r.z), labels_of(r.label), ptr(s.old_logp), ptr(s.advantage), ptr(s.ref_logp), ptr(o.loss),
-                                         ptr(o.more), stats, factor, ptr(o.dz), r.R, r.J, s.a, s.b, s.c, ws.data_ptr(), bytes,
-                                         stream_of(r.z));
+                                         ptr(o.more), stats, factor, ptr(o.dz), r.R, r.J, s.a, s.b, s.c, ws, bytes, stream_of(r.z));
   check(rc, s.name());
   return o;
 }
@@ -756,11 +756,13 @@ struct ChoiceLossFunction : torch::autograd::Function<ChoiceLossFunction> {
     ctx->saved_data["pairs"] = (int64_t)s->P;
     ctx->saved_data["gradient"] = c10::IValue::make_capsule(k);
     ctx->mark_non_differentiable({o.more});
+    ctx->set_materialize_grads(false);             // (else autograd fills zeros for `more`, a launch in every backward)
     return {o.loss, o.more};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const char* what = ctx->saved_data["pairs"].toInt() ? "preference_loss" : "policy_loss";
+    if (!grads[0].defined()) return {Tensor(), Tensor()};
     check_backward(saved[0], what);
     const Tensor g = as_cuda_f32(grads[0], "gradient of the loss");
     const auto k = c10::static_intrusive_pointer_cast<KeptGradient>(ctx->saved_data["gradient"].toCapsule());
@@ -771,7 +773,8 @@ struct ChoiceLossFunction : torch::autograd::Function<ChoiceLossFunction> {
     }
     if (!dz.defined()) {
       const int64_t R = saved[1].numel();
-      return {choice_backward(saved[0], saved[1], saved[2].narrow(0, 0, 2 * R), saved[2].narrow(0, 2 * R, R), g, what), Tensor()};
+      const float* stats = kept_stats(saved[2], R);
+      return {choice_backward(saved[0], saved[1], stats, stats + 2 * R, g, what), Tensor()};
     }
     const c10::cuda::CUDAGuard guard(dz.device());
     check(snntc_scale_gradient(ptr(dz), ptr(g), (size_t)dz.numel(), stream_of(dz)), what);
