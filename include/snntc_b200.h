@@ -192,8 +192,8 @@ SNNTC_API int snntc_sgdm_step(float* w, const float* g, float* vel, size_t n, fl
                               float grad_scale, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
- * The two ends of a network on tokens. None of these has a counterpart in the reference. Sizes N, V and R are 64-bit and
- * limited to 2^31-1 (V: 2^31-2); tensors may have more elements than that. Workspaces are 256-byte aligned.
+ * The two ends of a network on tokens. None of these has a counterpart in the reference. Sizes N, V and R are limited to 2^31-1
+ * (V: 2^31-2), J and D to 2^30; tensors may have more elements than that. Workspaces are 256-byte aligned.
  *
  * snntc_embedding_forward   y[N,D]: row t is scale * table[ids[t],:], or exp(scale * table[ids[t],:]) where `spikes` is not 0
  *                    (rows of spike times, encoded as snntc_encode does with one_minus = 0). Where ids[t] == padding or is

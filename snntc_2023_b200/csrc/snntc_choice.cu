@@ -143,11 +143,11 @@ policy_mean_kernel(const double3* terms, const double* inv_n, float* __restrict_
   }
 }
 
-// ---- rows. A group of G lanes (part of a warp, a warp, a CTA) holds a row in registers, NV vectors of four
-// a lane, all loads in flight at once: the row is read from memory once, and where the loss's factor follows from the row alone
-// (the policy loss), its gradient is written in the same pass. Rows of any length start anywhere, so a row is seen through the
-// 16-byte vectors that cover it; those that stick out at its ends are loaded and stored by element.
-// Maxima are a warp's own: every warp sums exp(x - its maximum), and one exchange joins (maximum, sum) pairs.
+// ---- rows. What bounds them is memory: 4 bytes read per logit, and 4 written where the gradient is formed. Where the loss's factor follows
+// from the row alone (the policy loss) the gradient is written in the pass that reads the row. Rows of any length start anywhere, so
+// a row is seen through the 16-byte vectors that cover it; those that stick out at its ends are loaded and stored by element.
+// Short rows stay in registers, NV vectors of four a lane, all loads in flight at once; long ones are streamed. Maxima are a lane's or a
+// warp's own: it sums exp(x - its maximum), and one exchange joins (maximum, sum) pairs.
 template <int NV>
 struct RowValues { float x[4 * NV]; };
 
@@ -626,7 +626,7 @@ int done() {
 
 int check_rows(long long R, int J) {
   if (R <= 0 || J <= 0) return SNNTC_E_SHAPE;
-  return R > 0x7fffffffLL ? SNNTC_E_TOO_LARGE : SNNTC_OK;
+  return R > 0x7fffffffLL || J > (1 << 30) ? SNNTC_E_TOO_LARGE : SNNTC_OK;   // (places in a row are 32-bit numbers)
 }
 
 // Longest row whose covering vectors fit `lanes` lanes of nv: rows that all start on 16 bytes fill them, others may begin three

@@ -106,8 +106,8 @@ __device__ __forceinline__ uint2 pair_at(const Keys& k, long long t) {
   return k.pairs ? ld_plain(k.pairs + t) : make_uint2(key_of(k.ids, t), (unsigned)t);
 }
 
-// 32 pairs to a CTA, a lane each; a warp counts in its eighth of the keys, four to a load that all lanes share. N^2 comparisons: 4096 pairs
-// are 1 us of them. An equal key counts where its position is lower.
+// 32 pairs to a CTA, a lane each; a warp counts in its eighth of the keys, four to a load that all lanes share. An equal key
+// counts where its position is lower. One launch against four: 300 pairs 4 us, 7007 15, where the passes take some 25.
 __global__ void __launch_bounds__(kThreads) sort_small_kernel(Ids ids, uint2* __restrict__ out, int N) {
   chain_wait();
   chain_next();
@@ -229,12 +229,14 @@ sort_scatter_kernel(Keys keys, const int* counts, uint2* __restrict__ out, long 
   }
 }
 
-// ---- sums of runs of equal keys. The sorted pairs are cut into tiles of M; a group of L lanes takes a tile and L vectors of the rows,
-// kTermsAhead rows of g in flight. Runs inside a tile are done there and then; of one that crosses a border the first tile leaves its
-// part in `tail`, the others theirs in `head`, and the joining kernel adds those in order. So a token that every second place holds is
-// summed by as many CTAs as its share, and the order of summation depends on the sizes alone.
-// Rows that no token names are zeroed by further CTAs of the same launch, a warp for 32 rows or a share of them: each lane looks
-// a row up in the sorted keys.
+// ---- sums of runs of equal keys. What bounds them is memory: g read once, the table's gradient written once (131 072 tokens of 512
+// values on as many rows: 537 MB in 92 us, 5.8 TB/s, behind 26 us of sort and before 8 us of joins).
+// The sorted pairs are cut into tiles of M; a group of L lanes takes a tile and L vectors of the rows, kTermsAhead rows of g in flight.
+// Runs inside a tile are done there and then; of one that crosses a border the first tile leaves its part in `tail`, the others theirs in
+// `head`, and the joining kernel adds those in order. So a token that every second place holds is summed by as many CTAs as its share,
+// and the order of summation depends on the sizes alone. (One CTA for each run: 8.3 ms, most of it the most frequent token's.)
+// Rows that no token names are zeroed by further CTAs of the same launch, a warp for 32 rows or a share of them: each lane looks a row up
+// in the sorted keys. (A clearing of the whole table in front would write the named rows twice.)
 constexpr int kTermsAhead = 8;
 constexpr int kSumTiles = 2048;           // at most, of rows that take a warp
 
@@ -284,7 +286,7 @@ __device__ void zero_rows(const RunSums& q) {
   const bool empty = v0 + lane < q.V && !(lo < end && ld_plain(&q.pairs[lo].x) == v0 + lane);
   unsigned todo = __ballot_sync(0xffffffffu, empty);
   while (todo) {                          // rows behind one another are one stretch of floats; this warp's share of it, in whole vectors
-    const int first = __ffs(todo) - 1, rows = __ffs(~(todo >> first)) - 1 < 0 ? 32 - first : __ffs(~(todo >> first)) - 1;
+    const int first = __ffs(todo) - 1, behind = __ffs(~(todo >> first)) - 1, rows = behind < 0 ? 32 : behind;   // (all 32: no bit behind them)
     todo &= rows == 32 ? 0u : ~(((1u << rows) - 1) << first);
     float* at = q.dtable + (v0 + first) * q.D;
     const long long n = (long long)rows * q.D;
@@ -349,14 +351,15 @@ __global__ void __launch_bounds__(kThreads) embed_join_kernel(RunSums q) {
   constexpr int kWarps = kThreads / 32, kFew = 8;
   __shared__ Vec<VEC> part[kWarps][32];
   __shared__ int last_tile[kWarps];        // of a run that is left to all; 0: none (a run's last tile is behind its first)
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.y * 32 + lane;
+  const int columns = (q.vectors + 31) / 32, tile0 = (int)(blockIdx.x / columns) * kWarps;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = (int)(blockIdx.x % columns) * 32 + lane;
   const auto head_of = [&](int t) { return Vec<VEC>::load(q.head + (long long)t * q.D + c * VEC); };
   const auto add = [](Vec<VEC>& sum, const Vec<VEC>& x) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) sum.v[j] += x.v[j];
   };
   {
-    const int tile = blockIdx.x * kWarps + warp;
+    const int tile = tile0 + warp;
     const long long i0 = (long long)tile * q.M, i1 = i0 + q.M;
     int last = 0;
     unsigned key = 0;
@@ -385,7 +388,7 @@ __global__ void __launch_bounds__(kThreads) embed_join_kernel(RunSums q) {
   }
   __syncthreads();
   for (int k = 0; k < kWarps; ++k) {
-    const int last = last_tile[k], tile = blockIdx.x * kWarps + k;
+    const int last = last_tile[k], tile = tile0 + k;
     if (last == 0) continue;
     Vec<VEC> sum = {};
     if (c < q.vectors)
@@ -413,7 +416,7 @@ int done() {
 int check_sizes(int id_bytes, long long N, long long V, int D) {
   if (N < 0 || V <= 0 || D <= 0) return SNNTC_E_SHAPE;
   if (id_bytes != 4 && id_bytes != 8) return SNNTC_E_PARAMS;
-  return N > 0x7fffffffLL || V >= 0x7fffffffLL ? SNNTC_E_TOO_LARGE : SNNTC_OK;
+  return N > 0x7fffffffLL || V >= 0x7fffffffLL || D > (1 << 30) ? SNNTC_E_TOO_LARGE : SNNTC_OK;   // (places in a row are 32-bit numbers)
 }
 
 bool by_four(int D, const void* a, const void* b, const void* c) {
@@ -472,7 +475,7 @@ int launch_sums(RunSums q, cudaStream_t s) {
   (void)launch_chained(embed_run_sums_kernel<VEC>, (unsigned)(q.sum_ctas + zero_ctas), kThreads, 0, s, 0, q);
   if (const int rc = done()) return rc;
   if (q.tiles == 1) return SNNTC_OK;
-  (void)launch_chained(embed_join_kernel<VEC>, dim3((q.tiles + 7) / 8, (q.vectors + 31) / 32), kThreads, 0, s, 0, q);
+  (void)launch_chained(embed_join_kernel<VEC>, (unsigned)((q.tiles + 7) / 8 * ((q.vectors + 31) / 32)), kThreads, 0, s, 0, q);
   return done();
 }
 

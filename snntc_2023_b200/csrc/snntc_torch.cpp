@@ -554,7 +554,11 @@ void check_backward(const Tensor& on, const char* what) {
   if (at::GradMode::is_enabled()) throw SnntcFailure(std::string(what) + ": the gradient cannot be differentiated again (create_graph)");
   const auto current = at::cuda::getCurrentCUDAStream(on.get_device());
   cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(current.stream(), &capturing) != cudaSuccess || capturing == cudaStreamCaptureStatusNone) return;
+  if (cudaStreamIsCapturing(current.stream(), &capturing) != cudaSuccess) {
+    (void)cudaGetLastError();     // (the legacy stream beside another thread's capture: not this call's to report)
+    return;
+  }
+  if (capturing == cudaStreamCaptureStatusNone) return;
   for (const torch::autograd::Edge& edge : torch::autograd::get_current_node()->next_edges()) {
     auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
     if (leaf == nullptr) continue;

@@ -13,7 +13,7 @@ def test_status_codes_of_the_embedding():
     fwd = lambda ids=FAKE, b=8, table=FAKE, y=FAKE, N=5, V=7, D=3: lib.snntc_embedding_forward(ids, b, table, y, N, V, D, 1.0, 0, -1, 1e5, 0)  # noqa: E731
     assert fwd(ids=0) == fwd(table=0) == fwd(y=0) == -1
     assert fwd(N=-1) == fwd(V=0) == fwd(D=0) == -2
-    assert fwd(N=1 << 31) == fwd(V=(1 << 31) - 1) == -4
+    assert fwd(N=1 << 31) == fwd(V=(1 << 31) - 1) == fwd(D=(1 << 30) + 1) == -4
     assert fwd(b=2) == -8
     assert fwd(N=0, ids=0, table=0, y=0) == 0
     size = lib.snntc_embedding_backward_workspace_bytes
@@ -31,7 +31,7 @@ def test_status_codes_of_the_losses_on_choices():
     lp = lambda z=FAKE, lab=FAKE, out=FAKE, R=4, J=3: lib.snntc_label_logp_forward(z, lab, out, 0, R, J, 0)  # noqa: E731
     assert lp(z=0) == lp(lab=0) == lp(out=0) == -1
     assert lp(R=0) == lp(J=0) == lp(R=-1) == -2
-    assert lp(R=1 << 31) == -4
+    assert lp(R=1 << 31) == lp(J=(1 << 30) + 1) == -4
     args = [FAKE] * 6
     for k in (0, 1, 2, 3, 5):
         a = list(args)
