@@ -217,15 +217,17 @@ struct Ends {
   }
 };
 
-// to = scale * exp(-row - top), less f at the label, for the vectors [v0, v1) and, with the row's first ones, its ends; zeros where f is 0.
-// By `lanes` lanes, U vectors at a time, from the last to the first. `to` is `apart` bytes behind the row.
-template <int U>
-__device__ __forceinline__ void grad_row(const float* row, ptrdiff_t apart, const Ends& e, int v0, int v1, int gl, int lanes, float top,
-                                         float scale, float f, int hot) {
-  const bool alike = (apart & 15) == 0;
-  const auto put = [&](const float4* from, float4 q) {
+// to = scale * exp(-row - top), less f at the label; zeros where f is 0. By `lanes` lanes, U vectors at a time, from the row's end to its
+// beginning. `to` is `apart` bytes behind the row.
+struct RowGradient {
+  const float* row;
+  ptrdiff_t apart;
+  Ends e;
+  float top, scale, f;
+  int hot;
+  __device__ __forceinline__ void put(const float4* from, float4 q) const {
     float* to = (float*)((char*)from + apart);
-    if (alike) {
+    if ((apart & 15) == 0) {
       __stcs((float4*)to, q);
     } else {
       to[0] = q.x;
@@ -233,30 +235,25 @@ __device__ __forceinline__ void grad_row(const float* row, ptrdiff_t apart, cons
       to[2] = q.z;
       to[3] = q.w;
     }
-  };
-  if (v0 == 0 && e.mine)
-    *(float*)((char*)(row + e.at) + apart) = f == 0.f ? 0.f : exp_term(-ld_plain(row + e.at) - top) * scale - (e.at == hot ? f : 0.f);
-  if (f == 0.f) {
-    for (int b = v0 + gl; b < v1; b += lanes) put(e.body + b, make_float4(0.f, 0.f, 0.f, 0.f));
-    return;
   }
-  const int hot_v = (hot - e.head) >> 2;
-  const float4* at = e.body + (v1 - 1 - gl);
-  for (int b = v1 - 1 - gl; b >= v0; b -= U * lanes, at -= U * lanes) {
+  // the vectors v, v - lanes, ...: U of them, or as many as there are down to the first
+  template <int U, bool ALL>
+  __device__ __forceinline__ void some(int v, int lanes) const {
+    const float4* at = e.body + v;
     float4 q[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       q[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (b - k * lanes >= v0) q[k] = __ldcs(at - k * lanes);
+      if (ALL || v - k * lanes >= 0) q[k] = __ldcs(at - k * lanes);
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      if (b - k * lanes < v0) break;
+      if (!ALL && v - k * lanes < 0) break;
       q[k].x = exp_term(-q[k].x - top) * scale;
       q[k].y = exp_term(-q[k].y - top) * scale;
       q[k].z = exp_term(-q[k].z - top) * scale;
       q[k].w = exp_term(-q[k].w - top) * scale;
-      if (b - k * lanes == hot_v) {
+      if (v - k * lanes == (hot - e.head) >> 2) {
         const int c = (hot - e.head) & 3;
         q[k].x -= c == 0 ? f : 0.f;
         q[k].y -= c == 1 ? f : 0.f;
@@ -266,7 +263,19 @@ __device__ __forceinline__ void grad_row(const float* row, ptrdiff_t apart, cons
       put(at - k * lanes, q[k]);
     }
   }
-}
+  template <int U>
+  __device__ __forceinline__ void all(int gl, int lanes) const {
+    if (e.mine) *(float*)((char*)(row + e.at) + apart) = f == 0.f ? 0.f : exp_term(-ld_plain(row + e.at) - top) * scale - (e.at == hot ? f : 0.f);
+    if (f == 0.f) {
+      for (int v = gl; v < e.vectors; v += lanes) put(e.body + v, make_float4(0.f, 0.f, 0.f, 0.f));
+      return;
+    }
+    int v = e.vectors - 1 - gl;
+    if (U > 2)
+      for (; v - (U - 1) * lanes >= 0; v -= U * lanes) some<U, true>(v, lanes);
+    for (; v >= 0; v -= 2 * lanes) some<2, false>(v, lanes);
+  }
+};
 
 template <int W>
 __device__ __forceinline__ float lanes_max(float m) {
@@ -279,6 +288,29 @@ __device__ __forceinline__ float lanes_sum(float s) {
 #pragma unroll
   for (int d = W / 2; d >= 1; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
   return s;
+}
+
+// The vectors at, at + stride, ... into a lane's running (maximum, sum): N of them, or as many as lie less than `left` behind the first
+template <int N, bool SHORT>
+__device__ __forceinline__ void absorb(const float4* at, int stride, int left, float& top, float& total) {
+  float x[4 * N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    float4 q = make_float4(CUDART_INF_F, CUDART_INF_F, CUDART_INF_F, CUDART_INF_F);
+    if (k * stride < left) q = ld_plain(at + k * stride);
+    x[4 * k] = -q.x;
+    x[4 * k + 1] = -q.y;
+    x[4 * k + 2] = -q.z;
+    x[4 * k + 3] = -q.w;
+  }
+  float m[4] = {top, -FLT_MAX, -FLT_MAX, -FLT_MAX}, s[4] = {};
+#pragma unroll
+  for (int k = 0; k < 4 * N; ++k) m[k % 4] = fmaxf(m[k % 4], x[k]);
+  const float t = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+#pragma unroll
+  for (int k = 0; k < 4 * N; ++k) s[k % 4] += sum_term<SHORT>(x[k] - t);
+  total = fmaf(total, expf(top - t), (s[0] + s[1]) + (s[2] + s[3]));
+  top = t;
 }
 
 struct RowOut {
@@ -375,7 +407,7 @@ template <int T, int G, int NV, bool HOLD, bool POLICY>
 __device__ __forceinline__ void rows_of_cta(const float* z, const long long* labels, const RowOut& out, const Policy& pol, long long R, int J,
                                             long long blk, double3* term) {
   static_assert(G <= 32 || G == T, "a row belongs to part of a warp, a warp or the CTA");
-  constexpr int kRows = T / G, W = G < 32 ? G : 32;
+  constexpr int kRows = T / G, W = G < 32 ? G : 32, kGradAhead = NV == 8 ? 8 : 2;
   __shared__ float2 stats[kRows > T / 32 ? kRows : T / 32];   // (top, total): of rows, or of a row's warps
   __shared__ float factors[kRows];
   const int tid = threadIdx.x, lane = tid & 31, gl = tid % G, own = tid / G;
@@ -409,24 +441,12 @@ __device__ __forceinline__ void rows_of_cta(const float* z, const long long* lab
     total = lanes_sum<W>((s[0] + s[1]) + (s[2] + s[3]));
   } else {
     if (live) {
-      for (int v0 = gl; v0 < e.vectors; v0 += NV * G) {
-#pragma unroll
-        for (int k = 0; k < NV; ++k) {
-          float4 q = make_float4(CUDART_INF_F, CUDART_INF_F, CUDART_INF_F, CUDART_INF_F);
-          if (v0 + k * G < e.vectors) q = ld_plain(e.body + v0 + k * G);
-          v.x[4 * k] = -q.x;
-          v.x[4 * k + 1] = -q.y;
-          v.x[4 * k + 2] = -q.z;
-          v.x[4 * k + 3] = -q.w;
-        }
-        float m[4] = {top, -FLT_MAX, -FLT_MAX, -FLT_MAX}, s[4] = {};
-#pragma unroll
-        for (int k = 0; k < 4 * NV; ++k) m[k % 4] = fmaxf(m[k % 4], v.x[k]);
-        const float t = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
-#pragma unroll
-        for (int k = 0; k < 4 * NV; ++k) s[k % 4] += sum_term<POLICY>(v.x[k] - t);
-        total = fmaf(total, expf(top - t), (s[0] + s[1]) + (s[2] + s[3]));
-        top = t;
+      int v0 = gl;
+      if (NV == 8) {
+        for (; v0 + (NV - 1) * G < e.vectors; v0 += NV * G) absorb<NV, POLICY>(e.body + v0, G, NV * G, top, total);
+        for (; v0 < e.vectors; v0 += 2 * G) absorb<2, POLICY>(e.body + v0, G, e.vectors - v0, top, total);
+      } else {
+        for (; v0 < e.vectors; v0 += NV * G) absorb<NV, POLICY>(e.body + v0, G, e.vectors - v0, top, total);
       }
       if (e.mine) {
         const float x = -ld_plain(row + e.at), t = fmaxf(top, x);
@@ -467,12 +487,12 @@ __device__ __forceinline__ void rows_of_cta(const float* z, const long long* lab
     for (int k = 0; k < 4 * NV; ++k) v.x[k] = f == 0.f ? 0.f : v.x[k] * scale;
     store_row<NV>(to, row, v, J, label, f, gl, G);
   } else {
-    grad_row<(T < 1024 ? 2 : NV)>(row, (char*)pol.dz - (char*)z, e, 0, e.vectors, gl, G, top, f == 0.f ? 0.f : f / total, f, (int)label);
+    RowGradient{row, (char*)pol.dz - (char*)z, e, top, f == 0.f ? 0.f : f / total, f, (int)label}.template all<kGradAhead>(gl, G);
   }
 }
 
 template <int T, int G, int NV, bool HOLD, bool POLICY>
-__global__ void __launch_bounds__(T, HOLD ? 1024 / T : 2048 / T)
+__global__ void __launch_bounds__(T, HOLD || NV == 8 ? 1024 / T : 2048 / T)
 choice_rows_kernel(const float* z, const long long* labels, RowOut out, Policy pol, long long R, int J) {
   chain_wait();
   chain_next();
@@ -540,7 +560,7 @@ choice_grad_kernel(const float* z, const long long* labels, const float2* stats,
     store_row<NV>(to, row, v, J, label, f, first, G);
   } else {
     const Ends e(row, J, gl);
-    grad_row<NV>(row, (char*)dz - (char*)z, e, 0, e.vectors, gl, G, st.x, scale, f, (int)label);
+    RowGradient{row, (char*)dz - (char*)z, e, st.x, scale, f, (int)label}.template all<NV>(gl, G);
   }
 }
 
@@ -642,13 +662,15 @@ struct Lanes {
   static constexpr int T = T_, G = G_, NV = NV_;
   static constexpr bool HOLD = HOLD_;
 };
-// Calls as() with the kernel's shape for rows of this length: the fewest lanes that hold one in eight vectors each, as every lane less shares the
-// row's numbers and shuffles among more rows (131 072 rows of 125: 37 us with a warp each, 14.6 with four lanes); beyond a warp's 1024
-// elements a warp that streams, then a CTA as large as leaves a lane some 32 elements: what follows a row's last load -- joins, its
-// numbers -- takes a CTA's time whatever its size (16 384 rows of 3001, with gradient: T = 128 85 us, 512 152; 8192 of 50 021: 779, 573
-// with 1024).
-template <typename As>
-auto by_length(const RowShape& w, int warp_row, As as) {
+// Calls as() with the kernel's shape for rows of this length: the fewest lanes that hold one in eight vectors each, as every lane less
+// shares the row's numbers and shuffles among more rows (131 072 rows of 125: 37 us with a warp each, 14.6 with four lanes). Beyond a
+// warp's 1024 elements, up to warp_row, a warp that streams; then a CTA, the larger the longer the row: what follows a row's last load --
+// joins, its numbers -- takes a CTA's time whatever its size, and the CTAs of an SM should be in different phases (16 384 rows of 3001 with
+// gradient: 128 threads 85 us, 512 152). Eight vectors in flight and half an SM's threads beat four and all of them, which leaves 32
+// registers a thread: 4096 rows of 26 000 71, 92 us. With gradient, what the CTAs of all SMs read must still be in L2 when it is read
+// again: few large ones from long_row on (4096 rows of 26 000: 256 threads 160 us, 512 178; of 32 768: 202, 182).
+template <int WARP_NV, typename As>
+auto by_length(const RowShape& w, int warp_row, int long_row, As as) {
   if (w.fits(1, 4)) return as(Lanes<256, 1, 4, true>{});
   if (w.fits(1, 8)) return as(Lanes<256, 1, 8, true>{});
   if (w.fits(2, 8)) return as(Lanes<256, 2, 8, true>{});
@@ -656,17 +678,17 @@ auto by_length(const RowShape& w, int warp_row, As as) {
   if (w.fits(8, 8)) return as(Lanes<256, 8, 8, true>{});
   if (w.fits(16, 8)) return as(Lanes<256, 16, 8, true>{});
   if (w.fits(32, 8)) return as(Lanes<256, 32, 8, true>{});
-  if (w.J <= warp_row) return as(Lanes<256, 32, 4, false>{});
+  if (w.J <= warp_row) return as(Lanes<256, 32, WARP_NV, false>{});
   if (w.J <= 6000) return as(Lanes<128, 128, 4, false>{});
   if (w.J <= 12000) return as(Lanes<256, 256, 4, false>{});
-  if (w.J <= 24000) return as(Lanes<512, 512, 4, false>{});
-  return as(Lanes<1024, 1024, 4, false>{});
+  if (w.J <= long_row) return as(Lanes<256, 256, 8, false>{});
+  return as(Lanes<512, 512, 8, false>{});
 }
 
 template <bool POLICY>
 int launch_rows(const float* z, const long long* labels, const RowOut& out, const Policy& pol, long long R, int J, cudaStream_t s,
                 unsigned* ctas = nullptr) {
-  return by_length(RowShape(z, J), POLICY ? 1800 : 6000, [&](auto lanes) {
+  return by_length<(POLICY ? 8 : 4)>(RowShape(z, J), POLICY ? 1800 : 6000, POLICY ? 28000 : 1 << 30, [&](auto lanes) {
     using L = decltype(lanes);
     constexpr int T = L::T, G = L::G;
     const unsigned grid = (unsigned)((R + T / G - 1) / (T / G));
@@ -679,7 +701,7 @@ int launch_rows(const float* z, const long long* labels, const RowOut& out, cons
 template <int T, int G, int NV, bool HOLD>
 int launch_grad_as(const float* z, const long long* labels, const float* stats, const float* factor, const float* gout, float* dz,
                    long long R, int J, cudaStream_t s) {
-  const int chunks = G == T ? (J + 3 + 4 * T * NV - 1) / (4 * T * NV) : 1;   // (up to three elements of the first vector are the row in front's)
+  const int chunks = G == T ? (J + RowShape(z, J).slack + 4 * T * NV - 1) / (4 * T * NV) : 1;
   const long long grid = G == T ? R * chunks : (R + T / G - 1) / (T / G);
   if (grid > 0x7fffffffLL) return SNNTC_E_TOO_LARGE;
   (void)launch_chained(choice_grad_kernel<T, G, NV, HOLD>, (unsigned)grid, T, 0, s, 0, z, labels, (const float2*)stats, factor, gout, dz, R, J, chunks);
@@ -704,7 +726,7 @@ int snntc_choice_backward(const float* z, const long long* labels, const float* 
   if (!z || !labels || !stats_2R || !factor || !dz) return SNNTC_E_NULL;
   if (const int rc = check_rows(R, J)) return rc;
   cudaStream_t s = (cudaStream_t)stream;
-  return by_length(RowShape(z, J), 1800, [&](auto lanes) {
+  return by_length<4>(RowShape(z, J), 1800, 0, [&](auto lanes) {
     using L = decltype(lanes);
     if constexpr (L::G == L::T) return launch_grad_as<128, 128, 4, true>(z, labels, stats_2R, factor, gout, dz, R, J, s);
     else return launch_grad_as<L::T, L::G, L::NV, L::HOLD>(z, labels, stats_2R, factor, gout, dz, R, J, s);
@@ -726,7 +748,7 @@ int snntc_policy_loss(const float* z, const long long* labels, const float* old_
   Policy pol{old_logp, advantage, ref_logp, inv_n, terms, dz, PolicyParams{1 - clip_low, 1 + clip_high, kl_coef}};
   const RowOut out{nullptr, nullptr, (float2*)stats_2R, factor};
   int rc = SNNTC_OK;
-  const bool small = by_length(RowShape(z, J), 0, [&](auto lanes) {
+  const bool small = by_length<4>(RowShape(z, J), 0, 0, [&](auto lanes) {
     using L = decltype(lanes);
     if constexpr (L::HOLD) {
       const long long blocks = (R + L::T / L::G - 1) / (L::T / L::G);

@@ -3,8 +3,8 @@ evaluations of their formulas.
 
 Tolerances, with u = 2^-24 (half a step of float32), d_j = -z_j - max(-z): a term exp(d_j) of a row's sum is off by the rounding of
 d_j, of log2(e) and of their product, 2.5 |d_j| u, and by the exponential's own 2^-22 = 4 u at most; the sum of a row by its longest chain of
-additions, 64 u for the row lengths here (a lane adds at most 32 and the tree over lanes has 10 levels), which weights the terms'
-errors by p_j. So total is off by REL = (4 + 64 + 2.5 sum_j p_j |d_j|) u relative, lp by REL + |lp| u (its own rounding),
+additions, 64 u for the row lengths here (a lane adds eight terms at a time, a long row's lanes some forty times, and the tree over
+lanes and warps has 10 levels), which weights the terms' errors by p_j. So total is off by REL = (4 + 64 + 2.5 sum_j p_j |d_j|) u relative, lp by REL + |lp| u (its own rounding),
 p_j by REL + (2.5 |d_j| + 4 + 3) u relative, and a gradient factor * (p - onehot) by |factor| (p_j * that + 2 u) where factor is exact."""
 import math
 
