@@ -199,9 +199,14 @@ SNNTC_API int snntc_sgdm_step(float* w, const float* g, float* vel, size_t n, fl
  *                    (rows of spike times, encoded as snntc_encode does with one_minus = 0). Where ids[t] == padding or is
  *                    outside [0, V): no_spike in all D places, and table is not read. ids: int32 or int64 (id_bytes 4 or 8).
  *                    N = 0 is a no-op.
+ * snntc_embedding_forward_sort  the same, and beside the lookup, on a library-owned stream where that is allowed
+ *                    (snntc_set_overlap), the sort of the tokens that the backward needs: `sorted` receives
+ *                    snntc_embedding_sorted_bytes(N, D) bytes, 256-byte aligned, which the caller keeps until then. Where that is
+ *                    0 (a short lookup) it is snntc_embedding_forward, and the backward sorts for itself.
  * snntc_embedding_backward  dtable[V,D] is written in full: the gradient of the table for the upstream gradient g[N,D], each row
  *                    summed over its tokens in the order of t (zeros where no token names it). `table` is read only where
- *                    `spikes` is not 0 and may be null otherwise. The same bits every run.
+ *                    `spikes` is not 0 and may be null otherwise. `sorted`: what snntc_embedding_forward_sort has left for the same
+ *                    ids, padding and V, and ids may be null; or null. The same bits every run, either way.
  *
  * For the losses z[R,J] are spike values (logits are -z) and labels[R] int64; a row whose label is outside [0, J) does not count:
  * its logits are not read, its log-probability is 0 and its gradient 0. stats_2R (R pairs of floats) receives what the backward
@@ -223,10 +228,15 @@ SNNTC_API int snntc_sgdm_step(float* w, const float* g, float* vel, size_t n, fl
  */
 SNNTC_API int snntc_embedding_forward(const void* ids, int id_bytes, const float* table, float* y, long long N, long long V, int D,
                                       float scale, int spikes, long long padding, float no_spike, void* stream);
+SNNTC_API size_t snntc_embedding_sorted_bytes(long long N, int D);
+SNNTC_API size_t snntc_embedding_sort_workspace_bytes(long long N, int D);
+SNNTC_API int snntc_embedding_forward_sort(const void* ids, int id_bytes, const float* table, float* y, long long N, long long V, int D,
+                                           float scale, int spikes, long long padding, float no_spike, void* sorted,
+                                           void* workspace, size_t workspace_bytes, void* stream);
 SNNTC_API size_t snntc_embedding_backward_workspace_bytes(long long N, long long V, int D);
-SNNTC_API int snntc_embedding_backward(const void* ids, int id_bytes, const float* g, const float* table, float* dtable, long long N,
-                                       long long V, int D, float scale, int spikes, long long padding, void* workspace,
-                                       size_t workspace_bytes, void* stream);
+SNNTC_API int snntc_embedding_backward(const void* ids, int id_bytes, const void* sorted, const float* g, const float* table,
+                                       float* dtable, long long N, long long V, int D, float scale, int spikes, long long padding,
+                                       void* workspace, size_t workspace_bytes, void* stream);
 SNNTC_API int snntc_label_logp_forward(const float* z, const long long* labels, float* logp, float* stats_2R, long long R, int J,
                                        void* stream);
 SNNTC_API int snntc_choice_backward(const float* z, const long long* labels, const float* stats_2R, const float* factor,

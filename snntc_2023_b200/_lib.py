@@ -50,7 +50,10 @@ SYMBOLS = {
     "snntc_sgdm_step": (_INT, [_F, _F, _F, _SZ] + [ctypes.c_float] * 3 + [_F]),
     "snntc_embedding_forward": (_INT, [_F, _INT, _F, _F, _LL, _LL, _INT, ctypes.c_float, _INT, _LL, ctypes.c_float, _F]),
     "snntc_embedding_backward_workspace_bytes": (_SZ, [_LL, _LL, _INT]),
-    "snntc_embedding_backward": (_INT, [_F, _INT, _F, _F, _F, _LL, _LL, _INT, ctypes.c_float, _INT, _LL, _F, _SZ, _F]),
+    "snntc_embedding_sorted_bytes": (_SZ, [_LL, _INT]),
+    "snntc_embedding_sort_workspace_bytes": (_SZ, [_LL, _INT]),
+    "snntc_embedding_forward_sort": (_INT, [_F, _INT, _F, _F, _LL, _LL, _INT, ctypes.c_float, _INT, _LL, ctypes.c_float, _F, _F, _SZ, _F]),
+    "snntc_embedding_backward": (_INT, [_F, _INT, _F, _F, _F, _F, _LL, _LL, _INT, ctypes.c_float, _INT, _LL, _F, _SZ, _F]),
     "snntc_label_logp_forward": (_INT, [_F] * 4 + [_LL, _INT, _F]),
     "snntc_choice_backward": (_INT, [_F] * 6 + [_LL, _INT, _F]),
     "snntc_policy_loss_workspace_bytes": (_SZ, [_LL]),

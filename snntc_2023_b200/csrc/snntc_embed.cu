@@ -7,12 +7,11 @@
 // The gradient sorts (id, position) pairs by id -- a least-significant-digit radix sort, stable, so that every id's positions
 // stay in order -- and sums runs of equal ids. No atomics on floats: the same bits every run.
 #include "../../include/snntc_b200.h"
+#include "snntc_common.cuh"
 #include "snntc_launch.cuh"
 
 #include <cuda_runtime.h>
 #include <stdint.h>
-
-namespace snntc { void count_launch(int n = 1); void note_cuda_error(cudaError_t e); }
 
 namespace {
 
@@ -449,18 +448,58 @@ int sum_tile(long long N, int D) {
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
+struct SortSpace {                      // of the radix sort, besides the sorted pairs
+  size_t other, counts, bytes;
+  explicit SortSpace(long long N, size_t at = 0) {
+    other = at;
+    counts = other + round256((size_t)N * sizeof(uint2));
+    bytes = counts + (size_t)kTiles * kDigits * sizeof(int);
+  }
+};
+
 struct BackwardSpace {
-  size_t pairs[2], counts, head, tail, bytes;
-  BackwardSpace(long long N, int D) {
+  size_t pairs, head, tail, bytes;
+  SortSpace sort;
+  BackwardSpace(long long N, int D) : pairs(0), sort(N, round256((size_t)N * sizeof(uint2))) {
     const size_t tiles = (size_t)((N + sum_tile(N, D) - 1) / sum_tile(N, D)), parts = round256(tiles * D * sizeof(float));
-    pairs[0] = 0;
-    pairs[1] = round256((size_t)N * sizeof(uint2));
-    counts = 2 * pairs[1];
-    head = counts + (size_t)kTiles * kDigits * sizeof(int);
+    head = sort.bytes;
     tail = head + parts;
     bytes = tail + parts;
   }
 };
+
+// The radix sort of the pairs: `sorted` receives them, `other` and `counts` are scratch. urgent: beside a kernel that fills the GPU, whose
+// CTAs still to come would otherwise all go first.
+int launch_sort(const Ids& ids, long long N, long long V, uint2* sorted, uint2* other, int* counts, bool urgent, cudaStream_t s) {
+  const SortPlan p = sort_plan(N, V);
+  int least = 0, greatest = 0;
+  if (urgent) (void)cudaDeviceGetStreamPriorityRange(&least, &greatest);
+  bool first = true;
+  const auto launch = [&](auto kernel, auto... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.tiles);
+    cfg.blockDim = dim3(kSortThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;      // (the kernels are written for it, see launch_chained)
+    attr[0].val.programmaticStreamSerializationAllowed = (long)p.tiles * kSortThreads <= snntc::kChainThreads && !(urgent && first);
+    first = false;                          // (what the first one on a stream of the library's waits for is an event)
+    attr[1].id = cudaLaunchAttributePriority;
+    attr[1].val.priority = greatest;
+    cfg.attrs = attr;
+    cfg.numAttrs = urgent ? 2 : 1;
+    (void)cudaLaunchKernelEx(&cfg, kernel, args...);
+    return done();
+  };
+  Keys keys{ids, nullptr};
+  for (int k = 0; k < p.passes; ++k) {
+    uint2* to = (p.passes - 1 - k) % 2 ? other : sorted;                  // the last pass's is `sorted`
+    if (const int rc = launch(sort_count_kernel, keys, counts, N, p.tile, p.bits * k, 1 << p.bits)) return rc;
+    if (const int rc = launch(sort_scatter_kernel, keys, (const int*)counts, to, N, p.tile, p.tiles, p.bits * k, 1 << p.bits)) return rc;
+    keys.pairs = to;
+  }
+  return SNNTC_OK;
+}
 
 template <int VEC>
 int launch_sums(RunSums q, cudaStream_t s) {
@@ -479,6 +518,24 @@ int launch_sums(RunSums q, cudaStream_t s) {
   return done();
 }
 
+// Whether the sort goes beside the lookup: that has to last for some time to hide it. us, lookup and gradient together, beside and one
+// after the other: 131 072 tokens of 512 values 173, 193, 20 000 of 1024 98, 102; 131 072 of 30 73, 69, 9000 of 64 73, 69 (the events).
+bool sorts_beside(long long N, int D) { return N > kSmallSort && N * D >= (4LL << 20); }
+
+int launch_lookup(const Ids& in, const float* table, float* y, long long N, int D, float scale, int spikes, float no_spike, cudaStream_t s) {
+  const bool four = by_four(D, table, y, nullptr);
+  const int vectors = four ? D / 4 : D;
+  int L = 1;                                // lanes to a row: up to a warp
+  while (L < 32 && L < vectors) L *= 2;
+  const auto launch = [&](auto kernel, int ahead) {
+    const long long rows = (long long)kThreads / L * ahead;
+    (void)launch_chained(kernel, (unsigned)((N + rows - 1) / rows), kThreads, 0, s, 0, in, table, y, N, D, vectors, L, scale, spikes, no_spike);
+    return done();
+  };
+  if (vectors <= 32) return four ? launch(embed_forward_kernel<4, 4, 1>, 4) : launch(embed_forward_kernel<1, 4, 1>, 4);
+  return four ? launch(embed_forward_kernel<4, 2, 2>, 2) : launch(embed_forward_kernel<1, 2, 2>, 2);
+}
+
 }  // namespace
 
 extern "C" {
@@ -488,19 +545,42 @@ int snntc_embedding_forward(const void* ids, int id_bytes, const float* table, f
   if (const int rc = check_sizes(id_bytes, N, V, D)) return rc;
   if (N == 0) return SNNTC_OK;
   if (!ids || !table || !y) return SNNTC_E_NULL;
-  const bool four = by_four(D, table, y, nullptr);
-  const int vectors = four ? D / 4 : D;
-  int L = 1;                                // lanes to a row: up to a warp
-  while (L < 32 && L < vectors) L *= 2;
+  return launch_lookup(Ids{ids, id_bytes == 8, V, padding}, table, y, N, D, scale, spikes, no_spike, (cudaStream_t)stream);
+}
+
+size_t snntc_embedding_sorted_bytes(long long N, int D) { return sorts_beside(N, D) ? (size_t)N * sizeof(uint2) : 0; }
+size_t snntc_embedding_sort_workspace_bytes(long long N, int D) { return sorts_beside(N, D) ? SortSpace(N).bytes : 0; }
+
+int snntc_embedding_forward_sort(const void* ids, int id_bytes, const float* table, float* y, long long N, long long V, int D, float scale,
+                                 int spikes, long long padding, float no_spike, void* sorted, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  if (!sorts_beside(N, D)) return snntc_embedding_forward(ids, id_bytes, table, y, N, V, D, scale, spikes, padding, no_spike, stream);
+  if (const int rc = check_sizes(id_bytes, N, V, D)) return rc;
+  if (!ids || !table || !y || !sorted) return SNNTC_E_NULL;
+  if (!workspace || (uintptr_t)workspace % 256 || (uintptr_t)sorted % 256 || workspace_bytes < snntc_embedding_sort_workspace_bytes(N, D))
+    return SNNTC_E_WORKSPACE;
+  cudaStream_t s = (cudaStream_t)stream, side = s;
   const Ids in{ids, id_bytes == 8, V, padding};
-  const auto launch = [&](auto kernel, int ahead) {
-    const long long rows = (long long)kThreads / L * ahead;
-    (void)launch_chained(kernel, (unsigned)((N + rows - 1) / rows), kThreads, 0, (cudaStream_t)stream, 0, in, table, y, N, D, vectors, L,
-                         scale, spikes, no_spike);
-    return done();
-  };
-  if (vectors <= 32) return four ? launch(embed_forward_kernel<4, 4, 1>, 4) : launch(embed_forward_kernel<1, 4, 1>, 4);
-  return four ? launch(embed_forward_kernel<4, 2, 2>, 2) : launch(embed_forward_kernel<1, 2, 2>, 2);
+  const SortSpace w(N);
+  snntc::AuxSlot* aux = snntc::aux_acquire(-1);
+  if (aux) {
+    const cudaError_t e = snntc::aux_fork(aux, s);
+    if (e != cudaSuccess) {
+      snntc::note_cuda_error(e);
+      return SNNTC_E_CUDA;
+    }
+    side = aux->stream;
+  }
+  int rc = launch_sort(in, N, V, (uint2*)sorted, (uint2*)((char*)workspace + w.other), (int*)((char*)workspace + w.counts), aux != nullptr, side);
+  if (rc == SNNTC_OK) rc = launch_lookup(in, table, y, N, D, scale, spikes, no_spike, s);
+  if (aux) {                                // on every path: a stream under capture must not be left forked
+    const cudaError_t e = snntc::aux_join(aux, s);
+    if (e != cudaSuccess && rc == SNNTC_OK) {
+      snntc::note_cuda_error(e);
+      rc = SNNTC_E_CUDA;
+    }
+  }
+  return rc;
 }
 
 size_t snntc_embedding_backward_workspace_bytes(long long N, long long V, int D) {
@@ -508,10 +588,11 @@ size_t snntc_embedding_backward_workspace_bytes(long long N, long long V, int D)
   return BackwardSpace(N, D).bytes;
 }
 
-int snntc_embedding_backward(const void* ids, int id_bytes, const float* g, const float* table, float* dtable, long long N, long long V,
-                             int D, float scale, int spikes, long long padding, void* workspace, size_t workspace_bytes, void* stream) {
+int snntc_embedding_backward(const void* ids, int id_bytes, const void* sorted, const float* g, const float* table, float* dtable,
+                             long long N, long long V, int D, float scale, int spikes, long long padding, void* workspace,
+                             size_t workspace_bytes, void* stream) {
   if (const int rc = check_sizes(id_bytes, N, V, D)) return rc;
-  if (!dtable || (N > 0 && (!ids || !g || (spikes && !table)))) return SNNTC_E_NULL;
+  if (!dtable || (N > 0 && ((!ids && !sorted) || !g || (spikes && !table)))) return SNNTC_E_NULL;
   if (N > 0 && (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < snntc_embedding_backward_workspace_bytes(N, V, D)))
     return SNNTC_E_WORKSPACE;
   cudaStream_t s = (cudaStream_t)stream;
@@ -522,26 +603,18 @@ int snntc_embedding_backward(const void* ids, int id_bytes, const float* g, cons
   }
   const BackwardSpace w(N, D);
   char* base = (char*)workspace;
-  uint2* pairs[2] = {(uint2*)(base + w.pairs[0]), (uint2*)(base + w.pairs[1])};
+  uint2* pairs = (uint2*)(base + w.pairs);
   const Ids in{ids, id_bytes == 8, V, padding};
-  Keys keys{in, nullptr};
-  if (N <= kSmallSort) {
-    (void)launch_chained(sort_small_kernel, (unsigned)((N + 31) / 32), kThreads, 0, s, 0, in, pairs[0], (int)N);
+  if (sorted) {
+    pairs = (uint2*)sorted;
+  } else if (N <= kSmallSort) {
+    (void)launch_chained(sort_small_kernel, (unsigned)((N + 31) / 32), kThreads, 0, s, 0, in, pairs, (int)N);
     if (const int rc = done()) return rc;
-    keys.pairs = pairs[0];
-  } else {
-    const SortPlan p = sort_plan(N, V);
-    int* counts = (int*)(base + w.counts);
-    for (int k = 0; k < p.passes; ++k) {
-      (void)launch_chained(sort_count_kernel, (unsigned)p.tiles, kSortThreads, 0, s, 0, keys, counts, N, p.tile, p.bits * k, 1 << p.bits);
-      if (const int rc = done()) return rc;
-      (void)launch_chained(sort_scatter_kernel, (unsigned)p.tiles, kSortThreads, 0, s, 0, keys, counts, pairs[k & 1], N, p.tile, p.tiles, p.bits * k, 1 << p.bits);
-      if (const int rc = done()) return rc;
-      keys.pairs = pairs[k & 1];
-    }
+  } else if (const int rc = launch_sort(in, N, V, pairs, (uint2*)(base + w.sort.other), (int*)(base + w.sort.counts), false, s)) {
+    return rc;
   }
   RunSums q = {};
-  q.pairs = keys.pairs;
+  q.pairs = pairs;
   q.g = g;
   q.table = table;
   q.dtable = dtable;

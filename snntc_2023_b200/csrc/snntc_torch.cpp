@@ -586,41 +586,59 @@ const void* id_ptr(const Tensor& ids, int* bytes) {
   return ids.data_ptr();
 }
 
-Tensor embed_forward_call(const Tensor& w, const Tensor& ids, const EmbedState& s) {
+// sorted, where given and where there are tokens enough, receives the sorted tokens for the backward
+Tensor embed_forward_call(const Tensor& w, const Tensor& ids, const EmbedState& s, Tensor* sorted = nullptr) {
   const c10::cuda::CUDAGuard guard(w.device());
   auto shape = ids.sizes().vec();
   shape.push_back(s.D);
   const Tensor y = empty_like_dev(shape, w);
   int bytes;
   const void* p = id_ptr(ids, &bytes);
-  check(snntc_embedding_forward(p, bytes, ptr(w), ptr(y), ids.numel(), s.V, to_int(s.D, "embedding"), (float)s.scale, s.spikes, s.padding,
-                                (float)s.no_spike, stream_of(w)), "embedding");
+  const int64_t N = ids.numel();
+  const int D = to_int(s.D, "embedding");
+  const size_t keep = sorted ? snntc_embedding_sorted_bytes(N, D) : 0;
+  int rc;
+  if (keep) {
+    *sorted = workspace(keep, w);
+    const size_t temporary = snntc_embedding_sort_workspace_bytes(N, D);
+    const Tensor ws = workspace(temporary, w);
+    rc = snntc_embedding_forward_sort(p, bytes, ptr(w), ptr(y), N, s.V, D, (float)s.scale, s.spikes, s.padding, (float)s.no_spike,
+                                      sorted->data_ptr(), ws.data_ptr(), temporary, stream_of(w));
+  } else {
+    rc = snntc_embedding_forward(p, bytes, ptr(w), ptr(y), N, s.V, D, (float)s.scale, s.spikes, s.padding, (float)s.no_spike, stream_of(w));
+  }
+  check(rc, "embedding");
   return y;
 }
 
 struct EmbedFunction : torch::autograd::Function<EmbedFunction> {
   static Tensor forward(AutogradContext* ctx, const Tensor& W, const Tensor& ids, c10::intrusive_ptr<EmbedState> s) {
     const Tensor w = W.contiguous();
+    Tensor sorted;
+    const Tensor y = embed_forward_call(w, ids, *s, &sorted);
     ctx->saved_data["call"] = c10::IValue::make_capsule(s);
-    if (s->spikes) ctx->save_for_backward({ids, w});
-    else ctx->save_for_backward({ids});
-    return embed_forward_call(w, ids, *s);
+    ctx->saved_data["sorted"] = sorted.defined();
+    const Tensor& tokens = sorted.defined() ? sorted : ids;
+    if (s->spikes) ctx->save_for_backward({tokens, w});
+    else ctx->save_for_backward({tokens});
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = c10::static_intrusive_pointer_cast<EmbedState>(ctx->saved_data["call"].toCapsule());
     const auto saved = ctx->get_saved_variables();
-    const Tensor& ids = saved[0];
+    const bool sorted = ctx->saved_data["sorted"].toBool();
     const Tensor g = as_cuda_f32(grads[0], "grad");
     const c10::cuda::CUDAGuard guard(g.device());
     if (!s->sink.defined()) check_backward(g, "embedding");
     const Tensor dw = s->sink.defined() ? s->sink : empty_like_dev({s->V, s->D}, g);
     const int D = to_int(s->D, "embedding");
-    const size_t bytes = snntc_embedding_backward_workspace_bytes(ids.numel(), s->V, D);
+    const int64_t N = g.numel() / D;
+    const size_t bytes = snntc_embedding_backward_workspace_bytes(N, s->V, D);
     const Tensor ws = workspace(bytes, g);
-    int id_bytes;
-    const void* p = id_ptr(ids, &id_bytes);
-    check(snntc_embedding_backward(p, id_bytes, ptr(g), s->spikes ? ptr(saved[1]) : nullptr, ptr(dw), ids.numel(), s->V, D, (float)s->scale,
-                                   s->spikes, s->padding, ws.data_ptr(), bytes, stream_of(g)), "embedding");
+    int id_bytes = 8;
+    const void* p = sorted ? nullptr : id_ptr(saved[0], &id_bytes);
+    check(snntc_embedding_backward(p, id_bytes, sorted ? saved[0].data_ptr() : nullptr, ptr(g), s->spikes ? ptr(saved[1]) : nullptr, ptr(dw),
+                                   N, s->V, D, (float)s->scale, s->spikes, s->padding, ws.data_ptr(), bytes, stream_of(g)), "embedding");
     return {s->sink.defined() ? Tensor() : dw, Tensor(), Tensor()};
   }
 };

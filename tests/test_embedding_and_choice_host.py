@@ -19,10 +19,18 @@ def test_status_codes_of_the_embedding():
     size = lib.snntc_embedding_backward_workspace_bytes
     assert size(0, 7, 3) == 0 and size(1000, 7, 3) >= 2 * 1000 * 8
     bwd = lambda ids=FAKE, g=FAKE, table=0, dt=FAKE, N=5, V=7, D=3, spikes=0, ws=FAKE, n=1 << 40: lib.snntc_embedding_backward(  # noqa: E731
-        ids, 8, g, table, dt, N, V, D, 1.0, spikes, -1, ws, n, 0)
+        ids, 8, 0, g, table, dt, N, V, D, 1.0, spikes, -1, ws, n, 0)
     assert bwd(ids=0) == bwd(g=0) == bwd(dt=0) == bwd(spikes=1) == -1
     assert bwd(N=-1) == bwd(V=0) == bwd(D=0) == -2
     assert bwd(ws=0) == bwd(ws=FAKE + 8) == bwd(n=size(5, 7, 3) - 1) == -5
+    kept, scratch = lib.snntc_embedding_sorted_bytes, lib.snntc_embedding_sort_workspace_bytes
+    assert kept(0, 9) == kept(8192, 9999) == scratch(8192, 9999) == kept(8193, 9) == 0   # a short lookup: the backward sorts
+    assert kept(8193, 512) == 8193 * 8 and scratch(8193, 512) > 8193 * 8
+    both = lambda ids=FAKE, table=FAKE, y=FAKE, out=FAKE, N=9000, ws=FAKE, n=1 << 40: lib.snntc_embedding_forward_sort(  # noqa: E731
+        ids, 8, table, y, N, 7, 512, 1.0, 0, -1, 1e5, out, ws, n, 0)
+    assert both(ids=0) == both(table=0) == both(y=0) == both(out=0) == -1
+    assert both(ws=0) == both(ws=FAKE + 8) == both(out=FAKE + 8) == both(n=scratch(9000, 512) - 1) == -5
+    assert both(N=0, ids=0, table=0, y=0, out=0, ws=0) == 0
 
 
 def test_status_codes_of_the_losses_on_choices():

@@ -49,7 +49,8 @@ def _check(ids, table, up, y, grad, scale, spikes, padding=None, no_spike=1e5):
 
 SIZES = [(1, 1, 1), (1, 10007, 784), (2, 2, 3), (31, 7, 4), (32, 1, 33), (33, 300, 128), (257, 255, 129), (257, 256, 64), (300, 257, 100),
          (1000, 65536, 12), (4097, 1000, 100), (5000, 3, 257), (7007, 50021, 129), (20000, 65535, 36), (40000, 131072, 8), (70001, 90, 16),
-         (3, 100, 5000), (65536, 1 << 20, 4), (40, 3, 2_100_001), (8192, 40, 7), (8193, 40, 8), (8200, 600, 31), (303_105, 513, 3), (150_000, 262_144, 2)]
+         (3, 100, 5000), (65536, 1 << 20, 4), (40, 3, 2_100_001), (8192, 40, 7), (8193, 40, 8), (8200, 600, 31), (303_105, 513, 3), (150_000, 262_144, 2), (8193, 1000, 512), (8500, 300_000, 515),
+         (40_000, 9, 128)]
 
 
 @pytest.mark.parametrize("N,V,D", SIZES)
@@ -177,11 +178,40 @@ def test_refusals():
         torch.autograd.grad(y.sum(), w, create_graph=True)
 
 
-def test_captured_replayed_and_on_another_stream():
+def test_the_sort_beside_the_lookup_is_the_backward_s_own():
+    """A lookup that is long enough sorts its tokens for the backward, on another stream where the library may: the same bits as
+    without that stream, and as from the C entry point that sorts in the backward. The ids are the caller's again after the lookup."""
+    import torch
+    from snntc_2023_b200 import _lib, ops
+    lib = _lib.load()
+    N, V, D = 30_011, 5000, 256
+    ids, table, up = _case(N, V, D, 3, skew=True)
+    ids[::50] = -1
+    w = table.clone().requires_grad_(True)
+    grads = []
+    for overlap in (1, 0):
+        lib.snntc_set_overlap(overlap)
+        try:
+            mine = ids.clone()
+            y = ops.snn_embedding(mine, w, scale=0.5, spikes=True)
+            mine.fill_(3)
+            grads.append(torch.autograd.grad(y, w, up)[0])
+        finally:
+            lib.snntc_set_overlap(1)
+    _check(ids, table, up, y.detach(), grads[0], 0.5, True)
+    out = torch.empty_like(table)
+    size = lib.snntc_embedding_backward_workspace_bytes(N, V, D)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    rc = lib.snntc_embedding_backward(ids.data_ptr(), 8, 0, up.data_ptr(), table.data_ptr(), out.data_ptr(), N, V, D, 0.5, 1, -1, ws.data_ptr(),
+                                      size, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(grads[0], grads[1]) and torch.equal(grads[0], out)
+
+
+@pytest.mark.parametrize("N,V,D", [(3001, 500, 36), (12_001, 700, 512)])
+def test_captured_replayed_and_on_another_stream(N, V, D):
     """Lookup and gradient captured once, replayed on other ids; and two streams at once: the results of plain calls."""
     import torch
     from snntc_2023_b200 import ops
-    N, V, D = 3001, 500, 36
     ids, table, up = _case(N, V, D, 1)
     w = table.clone().requires_grad_(True)
 
