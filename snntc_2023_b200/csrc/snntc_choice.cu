@@ -98,6 +98,12 @@ __device__ __forceinline__ double3 cluster_sum(double3 v) {
   cg::cluster_group cl = cg::this_cluster();
   v = block_sum(v);
   if (threadIdx.x == 0) mine = v;
+  if (cl.num_blocks() == 1) {
+    __syncthreads();
+    const double3 t = mine;
+    __syncthreads();
+    return t;
+  }
   cl.sync();
   double3 t = make_double3(0, 0, 0);
   for (unsigned k = 0; k < cl.num_blocks(); ++k) {
@@ -110,17 +116,35 @@ __device__ __forceinline__ double3 cluster_sum(double3 v) {
   return t;
 }
 
-// How many rows count. One cluster: 65 536 labels are eight loads a thread.
+// How many rows count, over a cluster, the same number in all threads
+__device__ __forceinline__ unsigned cluster_count(const long long* labels, long long R, int J) {
+  __shared__ unsigned part[32], mine;
+  cg::cluster_group cl = cg::this_cluster();
+  unsigned n = 0;
+#pragma unroll 8
+  for (long long r = (long long)blockIdx.x * blockDim.x + threadIdx.x; r < R; r += (long long)gridDim.x * blockDim.x)
+    n += counts(ld_plain(labels + r), J) ? 1u : 0u;
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = n;
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    n = __reduce_add_sync(0xffffffffu, threadIdx.x < blockDim.x / 32 ? part[threadIdx.x] : 0u);
+    if (threadIdx.x == 0) mine = n;
+  }
+  cl.sync();
+  n = 0;
+  for (unsigned k = 0; k < cl.num_blocks(); ++k) n += *cl.map_shared_rank(&mine, k);
+  cl.sync();
+  return n;
+}
+
+// One cluster: 65 536 labels are eight loads a thread.
 __global__ void __launch_bounds__(kSumThreads)
 policy_count_kernel(const long long* labels, double* __restrict__ inv_n, long long R, int J) {
   chain_wait();
   chain_next();
-  double3 n = make_double3(0, 0, 0);
-#pragma unroll 8
-  for (long long r = (long long)blockIdx.x * kSumThreads + threadIdx.x; r < R; r += (long long)gridDim.x * kSumThreads)
-    n.x += counts(ld_plain(labels + r), J) ? 1.0 : 0.0;
-  n = cluster_sum(n);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *inv_n = n.x > 0 ? 1.0 / n.x : 0.0;
+  const unsigned n = cluster_count(labels, R, J);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *inv_n = n > 0 ? 1.0 / n : 0.0;
 }
 
 __global__ void __launch_bounds__(kSumThreads)
@@ -509,10 +533,9 @@ policy_small_kernel(const float* z, const long long* labels, RowOut out, Policy 
   chain_next();
   __shared__ double inv_n;
   __shared__ double3 term;
-  double3 n = make_double3(0, 0, 0), sum = n;
-  for (long long r = (long long)blockIdx.x * T + threadIdx.x; r < R; r += (long long)gridDim.x * T) n.x += counts(ld_plain(labels + r), J) ? 1.0 : 0.0;
-  n = cluster_sum(n);
-  const double inv = n.x > 0 ? 1.0 / n.x : 0.0;
+  double3 sum = make_double3(0, 0, 0);
+  const unsigned n = cluster_count(labels, R, J);
+  const double inv = n > 0 ? 1.0 / n : 0.0;
   if (threadIdx.x == 0) inv_n = inv;
   __syncthreads();
   pol.inv_n = &inv_n;
@@ -672,12 +695,12 @@ struct Lanes {
 template <int WARP_NV, typename As>
 auto by_length(const RowShape& w, int warp_row, int long_row, As as) {
   if (w.fits(1, 4)) return as(Lanes<256, 1, 4, true>{});
-  if (w.fits(1, 8)) return as(Lanes<256, 1, 8, true>{});
-  if (w.fits(2, 8)) return as(Lanes<256, 2, 8, true>{});
-  if (w.fits(4, 8)) return as(Lanes<256, 4, 8, true>{});
-  if (w.fits(8, 8)) return as(Lanes<256, 8, 8, true>{});
-  if (w.fits(16, 8)) return as(Lanes<256, 16, 8, true>{});
-  if (w.fits(32, 8)) return as(Lanes<256, 32, 8, true>{});
+  if (w.fits(1, 8)) return as(Lanes<128, 1, 8, true>{});
+  if (w.fits(2, 8)) return as(Lanes<128, 2, 8, true>{});
+  if (w.fits(4, 8)) return as(Lanes<128, 4, 8, true>{});
+  if (w.fits(8, 8)) return as(Lanes<128, 8, 8, true>{});
+  if (w.fits(16, 8)) return as(Lanes<128, 16, 8, true>{});
+  if (w.fits(32, 8)) return as(Lanes<128, 32, 8, true>{});
   if (w.J <= warp_row) return as(Lanes<256, 32, WARP_NV, false>{});
   if (w.J <= 6000) return as(Lanes<128, 128, 4, false>{});
   if (w.J <= 12000) return as(Lanes<256, 256, 4, false>{});
