@@ -686,9 +686,9 @@ Rows choice_rows(const Tensor& logit, const Tensor& label, const char* what) {
 }
 const long long* labels_of(const Tensor& t) { return (const long long*)t.data_ptr<int64_t>(); }
 
-Tensor constant(const Tensor& t, const Tensor& like, int64_t n, const char* name) {
+Tensor constant(const Tensor& t, const Tensor& like, at::IntArrayRef shape, const char* name) {
   const Tensor c = on_device(as_cuda_f32(t, name), like, name);
-  TORCH_CHECK_VALUE(c.numel() == n, name, " must hold ", n, " values, got ", c.numel());
+  TORCH_CHECK_VALUE(c.sizes() == shape, name, " must have the shape ", shape, ", got ", c.sizes());
   TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && t.requires_grad()), name, " is a constant of the loss: detach it");
   return c;
 }
@@ -820,9 +820,9 @@ std::pair<Tensor, Tensor> policy_loss(const Tensor& logit, const Tensor& label, 
   TORCH_CHECK_VALUE(kl_coef == 0 || ref_logp.has_value(), "policy_loss: the KL term needs ref_logp");
   auto s = c10::make_intrusive<ChoiceState>();
   s->rows = choice_rows(logit, label, "policy_loss");
-  s->old_logp = constant(old_logp, s->rows.z, s->rows.R, "old_logp");
-  s->advantage = constant(advantage, s->rows.z, s->rows.R, "advantage");
-  if (ref_logp.has_value()) s->ref_logp = constant(*ref_logp, s->rows.z, s->rows.R, "ref_logp");
+  s->old_logp = constant(old_logp, s->rows.z, label.sizes(), "old_logp");
+  s->advantage = constant(advantage, s->rows.z, label.sizes(), "advantage");
+  if (ref_logp.has_value()) s->ref_logp = constant(*ref_logp, s->rows.z, label.sizes(), "ref_logp");
   s->a = clip_low;
   s->b = clip_high;
   s->c = kl_coef;
@@ -846,7 +846,7 @@ std::pair<Tensor, Tensor> preference_loss(const Tensor& logit, const Tensor& lab
     TORCH_CHECK_VALUE(logit.dim() >= 3 && texts % 2 == 0, "preference_loss: without starts, logit is [2 * pairs, rows, classes]");
   }
   s->P = to_int(texts / 2, "preference_loss");
-  if (ref_logp.has_value()) s->ref_logp = constant(*ref_logp, s->rows.z, texts, "ref_logp");
+  if (ref_logp.has_value()) s->ref_logp = constant(*ref_logp, s->rows.z, {texts}, "ref_logp");
   s->a = beta;
   s->b = smoothing;
   return choice_loss(logit, s);

@@ -45,7 +45,7 @@ def constraint_cost(weights, K, K2):
 
 def label_log_probs(logit, label):
     """log softmax(-logit)[label] of every row: logit [..., classes] spike values, label [...] integers; [...]. A row whose label
-    is outside the classes (-1, say) does not count: 0, and no gradient. Under no_grad this is what policy_loss and
+    is outside the classes (-1, say) does not count: 0, and no gradient. The gradient cannot be differentiated again. Under no_grad this is what policy_loss and
     preference_loss take as the old and the reference network's log-probabilities."""
     return _lib.native().label_log_probs(_tensor(logit, "logit"), _tensor(label, "label"))
 
@@ -56,8 +56,9 @@ def policy_loss(logit, label, old_logp, advantage, ref_logp=None, clip_low=0.2, 
         -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * k
         r = exp(lp - old_logp), A = advantage, k = exp(ref_logp - lp) - (ref_logp - lp) - 1, lp = label_log_probs(logit, label)
 
-    logit [..., classes]; label, old_logp, advantage, ref_logp one value per row, the last three constants. with_stats=True
-    also returns [mean k, share of rows whose ratio was clipped]."""
+    logit [..., classes]; label, old_logp, advantage, ref_logp [...], one value per row, the last three constants. with_stats=True
+    also returns [mean k, share of rows whose ratio was clipped]. The gradient is formed with the loss, in the pass that reads the
+    logits; it cannot be differentiated again."""
     loss, stats = _lib.native().policy_loss(_tensor(logit, "logit"), _tensor(label, "label"), _tensor(old_logp, "old_logp"),
                                             _tensor(advantage, "advantage"),
                                             None if ref_logp is None else _tensor(ref_logp, "ref_logp"), float(clip_low),
@@ -74,7 +75,8 @@ def preference_loss(logit, label, starts=None, ref_logp=None, beta=0.1, label_sm
     Texts one behind the other: logit [rows, classes], label [rows], `starts` 2P+1 ascending offsets on the GPU, text s being
     rows starts[s] to starts[s+1] (rows behind the last are of no text). Padded texts: logit [2P, rows, classes], label
     [2P, rows], no starts. Rows whose label is outside the classes (prompts, padding) do not count. ref_logp [2P]: the
-    reference network's sums (none: 0), a constant. with_margins=True also returns the m_k."""
+    reference network's sums (none: 0), a constant. with_margins=True also returns the m_k. The gradient cannot be differentiated
+    again."""
     loss, margins = _lib.native().preference_loss(_tensor(logit, "logit"), _tensor(label, "label"),
                                                   None if starts is None else _tensor(starts, "starts"),
                                                   None if ref_logp is None else _tensor(ref_logp, "ref_logp"), float(beta),

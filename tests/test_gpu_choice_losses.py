@@ -300,6 +300,33 @@ def test_infinite_and_nan_outputs():
         assert lp[3].isnan() and z1.grad[3, 1].isnan()
 
 
+@pytest.mark.parametrize("J", [9, 120, 900, 3500, 30000])
+def test_outputs_masked_by_the_largest_value(J):
+    """Classes switched off by the largest float: no part in a softmax, the row that has nothing else is uniform; and the lowest value,
+    beside which everything else is nothing."""
+    import torch
+    from snntc_2023_b200 import train
+    most = torch.finfo(torch.float32).max
+    z, lab = _logits(5, J, J + 1, ignore=0.0)
+    z[1:, J // 2:] = most
+    lab[1:] = 0
+    z[3] = most
+    z[4, 0] = -most
+    z1 = z.clone().requires_grad_(True)
+    lp = train.label_log_probs(z1, lab)
+    lp.sum().backward()
+    assert abs(float(lp[3].detach()) + math.log(J)) < 1e-5 * math.log(J) and float(lp[4].detach()) == 0.0
+    assert not z1.grad[1:3, J // 2:].any() and not z1.grad[4].any()
+    keep = [0, 1, 2]
+    ref = Ref(z[keep].clamp(max=1e30), lab[keep])
+    ref.check_lp(lp.detach()[keep])
+    ref.check_grad(z1.grad[keep], torch.ones(3, dtype=torch.float64, device="cuda"), torch.zeros(3, dtype=torch.float64, device="cuda"))
+    old = lp.detach() - 0.01
+    loss = train.policy_loss(z1, lab, old, torch.ones(5, device="cuda"), ref_logp=old, kl_coef=0.1)
+    (grad,) = torch.autograd.grad(loss, z1)
+    assert loss.isfinite() and grad.isfinite().all()
+
+
 def test_gradients_against_differences():
     """Central differences of the losses in float64 (their formulas' own, at the kernels' inputs) along random directions: with steps of
     1e-6 they are good to 1e-7 of the slope's size."""
@@ -408,6 +435,11 @@ def test_refusals():
         train.policy_loss(z, lab, v[:7], v)
     with pytest.raises(ValueError):
         train.policy_loss(z, lab, v, v.double())
+    for bad in (v.view(4, 2), v[:1], v[0]):                               # as many values in another shape, or to be broadcast
+        with pytest.raises(ValueError):
+            train.policy_loss(z, lab, v, bad)
+    with pytest.raises(ValueError):
+        train.policy_loss(z.view(2, 4, 5), lab.view(2, 4), v.view(4, 2), v.view(2, 4))
     with pytest.raises(_lib.SnntcError):
         train.policy_loss(z, lab, v.cpu(), v)
     with pytest.raises(ValueError, match="detach"):
@@ -435,6 +467,54 @@ def test_refusals():
         z1 += 1
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+def test_a_loss_used_twice_and_beside_others():
+    """One node, one backward: the factors of a loss that enters an objective twice add up before its kernel runs; beside another loss of
+    the same logits the gradients are added."""
+    import torch
+    from snntc_2023_b200 import train
+    z, lab = _logits(40, 30, 8)
+    adv = torch.randn(40, device="cuda")
+    old = train.label_log_probs(z, lab) - 0.1
+    z1 = z.clone().requires_grad_(True)
+    loss = train.policy_loss(z1, lab, old, adv)
+    other = train.loss_func(z1, lab.clamp(min=0))
+    (alone,) = torch.autograd.grad(loss, z1, retain_graph=True)           # hands the kept gradient out
+    mine = alone.clone()
+    (ce,) = torch.autograd.grad(other, z1, retain_graph=True)
+    alone.zero_()                                                         # (the caller's: nothing of it is read again)
+    (both,) = torch.autograd.grad(loss * 3.0 + loss + other, z1)
+    assert torch.allclose(both, 4.0 * mine + ce, rtol=1e-5, atol=1e-9)
+
+
+def test_two_threads_at_once():
+    """Both directions of every loss from two host threads on streams of their own: the results of calls one after the other."""
+    import threading
+
+    import torch
+    cases = []
+    for k, (R, J) in enumerate(((300, 40), (64, 9000))):
+        z, lab = _logits(R, J, 70 + k)
+        cases.append((z, lab, -2 - torch.rand(R, device="cuda"), torch.randn(R, device="cuda"), -2 - torch.rand(R, device="cuda"),
+                      torch.tensor([0, R // 4, R // 2, R // 2, R], device="cuda")))
+    plain = [_all_losses(c[0].clone().requires_grad_(True), *c[1:]) for c in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = _all_losses(cases[k][0].clone().requires_grad_(True), *cases[k][1:])
+                torch.cuda.current_stream().synchronize()
+                bad.extend(1 for a, b in zip(got, plain[k]) if not torch.equal(a, b))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 def _all_losses(z, lab, old, adv, refp, starts):

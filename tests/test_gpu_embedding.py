@@ -157,6 +157,71 @@ def test_a_table_beyond_32_bit_offsets():
     assert not grad.any()
 
 
+def test_more_than_32_bits_of_values():
+    """2.2e9 values of 2.2 million tokens. Upstream ones: a row's gradient is the number of its tokens, exactly."""
+    import torch
+    from snntc_2023_b200 import ops
+    N, V, D = 2_200_003, 300, 1000
+    ids = torch.randint(0, V, (N,), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    w = torch.rand(V, D, device="cuda").requires_grad_(True)
+    y = ops.snn_embedding(ids, w)
+    for t in (0, 1, N // 2, N - 2, N - 1):
+        assert torch.equal(y[t].detach(), w.detach()[ids[t]])
+    (grad,) = torch.autograd.grad(y, w, torch.ones_like(y))
+    assert torch.equal(grad, torch.bincount(ids, minlength=V).float()[:, None].expand(V, D))
+
+
+def test_one_id_without_a_shape_and_arrays_by_dlpack():
+    import torch
+    from snntc_2023_b200 import ops
+
+    class Array:
+        def __init__(self, t):
+            self.t = t
+
+        def __dlpack__(self, **kw):
+            return self.t.__dlpack__(**kw)
+
+        def __dlpack_device__(self):
+            return self.t.__dlpack_device__()
+
+    w = torch.rand(5, 7, device="cuda")
+    assert torch.equal(ops.snn_embedding(torch.tensor(3, device="cuda"), w, scale=2.0), 2.0 * w[3])
+    assert torch.equal(ops.snn_embedding(Array(torch.tensor([4, 1], device="cuda")), Array(w)), w[[4, 1]])
+
+
+def test_two_threads_at_once():
+    """Lookup, sort and gradient from two host threads on streams of their own."""
+    import threading
+
+    import torch
+    from snntc_2023_b200 import ops
+    cases = [_case(12_000, 3000, 400, 1), _case(500, 90, 33, 2)]
+
+    def call(ids, table, up):
+        w = table.clone().requires_grad_(True)
+        y = ops.snn_embedding(ids, w, spikes=True)
+        return y.detach(), torch.autograd.grad(y, w, up)[0]
+
+    plain = [call(*c) for c in cases]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(k):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = call(*cases[k])
+                torch.cuda.current_stream().synchronize()
+                bad.extend(1 for a, b in zip(got, plain[k]) if not torch.equal(a, b))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
 def test_refusals():
     import torch
     from snntc_2023_b200 import ops
