@@ -18,6 +18,8 @@
 #include <math_constants.h>
 #include <stdint.h>
 
+#include <utility>
+
 namespace snntc { void count_launch(int n = 1); void note_cuda_error(cudaError_t e); }
 
 namespace {
@@ -27,6 +29,7 @@ using snntc::chain_next;
 using snntc::chain_wait;
 using snntc::launch_chained;
 using snntc::ld_plain;
+using snntc::ld_stream_at;
 
 __device__ __forceinline__ bool counts(long long label, int J) { return label >= 0 && label < J; }
 
@@ -241,7 +244,7 @@ struct Ends {
   }
 };
 
-// to = scale * exp(-row - top), less f at the label; zeros where f is 0. By `lanes` lanes, U vectors at a time, from the row's end to its
+// to = scale * exp(-row - top), less f at the label; zeros where f is 0. By LANES lanes, U vectors at a time, from the row's end to its
 // beginning. `to` is `apart` bytes behind the row.
 struct RowGradient {
   const float* row;
@@ -260,44 +263,39 @@ struct RowGradient {
       to[3] = q.w;
     }
   }
-  // the vectors v, v - lanes, ...: U of them, or as many as there are down to the first
-  template <int U, bool ALL>
-  __device__ __forceinline__ void some(int v, int lanes) const {
+  // the vectors v, v - LANES, ...: all of the K, or as many as there are down to the first
+  template <int LANES, bool ALL, int... K>
+  __device__ __forceinline__ void some(int v, std::integer_sequence<int, K...>) const {
     const float4* at = e.body + v;
-    float4 q[U];
+    float4 q[sizeof...(K)] = {(ALL || v - K * LANES >= 0 ? ld_stream_at<-K * LANES * 16>(at, scale) : make_float4(0.f, 0.f, 0.f, 0.f))...};
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      q[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (ALL || v - k * lanes >= 0) q[k] = __ldcs(at - k * lanes);
-    }
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (!ALL && v - k * lanes < 0) break;
+    for (int k = 0; k < (int)sizeof...(K); ++k) {
+      if (!ALL && v - k * LANES < 0) break;
       q[k].x = exp_term(-q[k].x - top) * scale;
       q[k].y = exp_term(-q[k].y - top) * scale;
       q[k].z = exp_term(-q[k].z - top) * scale;
       q[k].w = exp_term(-q[k].w - top) * scale;
-      if (v - k * lanes == (hot - e.head) >> 2) {
+      if (v - k * LANES == (hot - e.head) >> 2) {
         const int c = (hot - e.head) & 3;
         q[k].x -= c == 0 ? f : 0.f;
         q[k].y -= c == 1 ? f : 0.f;
         q[k].z -= c == 2 ? f : 0.f;
         q[k].w -= c == 3 ? f : 0.f;
       }
-      put(at - k * lanes, q[k]);
+      put(at - k * LANES, q[k]);
     }
   }
-  template <int U>
-  __device__ __forceinline__ void all(int gl, int lanes) const {
+  template <int LANES, int U>
+  __device__ __forceinline__ void all(int gl) const {
     if (e.mine) *(float*)((char*)(row + e.at) + apart) = f == 0.f ? 0.f : exp_term(-ld_plain(row + e.at) - top) * scale - (e.at == hot ? f : 0.f);
     if (f == 0.f) {
-      for (int v = gl; v < e.vectors; v += lanes) put(e.body + v, make_float4(0.f, 0.f, 0.f, 0.f));
+      for (int v = gl; v < e.vectors; v += LANES) put(e.body + v, make_float4(0.f, 0.f, 0.f, 0.f));
       return;
     }
     int v = e.vectors - 1 - gl;
     if (U > 2)
-      for (; v - (U - 1) * lanes >= 0; v -= U * lanes) some<U, true>(v, lanes);
-    for (; v >= 0; v -= 2 * lanes) some<2, false>(v, lanes);
+      for (; v - (U - 1) * LANES >= 0; v -= U * LANES) some<LANES, true>(v, std::make_integer_sequence<int, U>());
+    for (; v >= 0; v -= 2 * LANES) some<LANES, false>(v, std::make_integer_sequence<int, 2>());
   }
 };
 
@@ -511,7 +509,7 @@ __device__ __forceinline__ void rows_of_cta(const float* z, const long long* lab
     for (int k = 0; k < 4 * NV; ++k) v.x[k] = f == 0.f ? 0.f : v.x[k] * scale;
     store_row<NV>(to, row, v, J, label, f, gl, G);
   } else {
-    RowGradient{row, (char*)pol.dz - (char*)z, e, top, f == 0.f ? 0.f : f / total, f, (int)label}.template all<kGradAhead>(gl, G);
+    RowGradient{row, (char*)pol.dz - (char*)z, e, top, f == 0.f ? 0.f : f / total, f, (int)label}.template all<G, kGradAhead>(gl);
   }
 }
 
@@ -583,7 +581,7 @@ choice_grad_kernel(const float* z, const long long* labels, const float2* stats,
     store_row<NV>(to, row, v, J, label, f, first, G);
   } else {
     const Ends e(row, J, gl);
-    RowGradient{row, (char*)dz - (char*)z, e, st.x, scale, f, (int)label}.template all<NV>(gl, G);
+    RowGradient{row, (char*)dz - (char*)z, e, st.x, scale, f, (int)label}.template all<G, NV>(gl);
   }
 }
 

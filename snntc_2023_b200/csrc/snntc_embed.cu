@@ -19,6 +19,7 @@ using snntc::chain_next;
 using snntc::chain_wait;
 using snntc::launch_chained;
 using snntc::ld_plain;
+using snntc::ld_stream;
 
 // Ids of 32 or 64 bits; what is no token of the table becomes V, the largest key.
 struct Ids {
@@ -38,7 +39,7 @@ template <int VEC> struct Vec;
 template <> struct Vec<1> {
   float v[1];
   static __device__ __forceinline__ Vec load(const float* p) { return {{ld_plain(p)}}; }
-  static __device__ __forceinline__ Vec load_once(const float* p) { return {{__ldcs(p)}}; }
+  static __device__ __forceinline__ Vec load_once(const float* p) { return {{ld_stream(p)}}; }
   __device__ __forceinline__ void store(float* p) const { *p = v[0]; }
   __device__ __forceinline__ void store_once(float* p) const { __stcs(p, v[0]); }
 };
@@ -46,7 +47,7 @@ template <> struct Vec<4> {
   float v[4];
   static __device__ __forceinline__ Vec of(float4 q) { return {{q.x, q.y, q.z, q.w}}; }
   static __device__ __forceinline__ Vec load(const float* p) { return of(ld_plain((const float4*)p)); }
-  static __device__ __forceinline__ Vec load_once(const float* p) { return of(__ldcs((const float4*)p)); }
+  static __device__ __forceinline__ Vec load_once(const float* p) { return of(ld_stream((const float4*)p)); }
   __device__ __forceinline__ void store(float* p) const { *(float4*)p = make_float4(v[0], v[1], v[2], v[3]); }
   __device__ __forceinline__ void store_once(float* p) const { __stcs((float4*)p, make_float4(v[0], v[1], v[2], v[3])); }
 };

@@ -50,6 +50,21 @@ __device__ __forceinline__ float ld_stream(const float* p) {
   asm volatile("ld.global.cs.f32 %0, [%1];" : "=f"(v) : "l"(__cvta_generic_to_global(p)));
   return v;
 }
+__device__ __forceinline__ float4 ld_stream(const float4* p) {
+  float4 v;
+  asm volatile("ld.global.cs.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(__cvta_generic_to_global(p)));
+  return v;
+}
+// The same at a fixed distance in bytes, free to move among other instructions but not in front of what `behind` was formed from: a value
+// that was loaded behind chain_wait().
+template <int BYTES>
+__device__ __forceinline__ float4 ld_stream_at(const float4* p, float behind) {
+  float4 v;
+  asm("ld.global.cs.v4.f32 {%0, %1, %2, %3}, [%4 + %5]; // %6"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(__cvta_generic_to_global(p)), "n"(BYTES), "f"(behind));
+  return v;
+}
 
 // A grid, and whether it may be launched as a dependent (the kernel is written for it either way).
 struct ChainGrid {
