@@ -46,7 +46,7 @@ template <bool SHORT>
 __device__ __forceinline__ float sum_term(float d) { return SHORT ? exp_term(d) : expf(d); }
 
 constexpr int kSumThreads = 1024;
-constexpr int kFewPairs = 16;        // two for each CTA of a cluster
+constexpr int kFewPairs = 8;         // one for each CTA of a cluster (8 pairs: 7 us against 8.5 with a launch for the mean, 12: 9.4, 8.3)
 constexpr int kSmallBlocks = 16;     // CTAs' worth of rows for a policy loss by one cluster
 
 __device__ __forceinline__ double label_logp(float z_label, float2 st) {
@@ -683,13 +683,18 @@ struct Lanes {
   static constexpr int T = T_, G = G_, NV = NV_;
   static constexpr bool HOLD = HOLD_;
 };
-// Calls as() with the kernel's shape for rows of this length: the fewest lanes that hold one in eight vectors each, as every lane less
-// shares the row's numbers and shuffles among more rows (131 072 rows of 125: 37 us with a warp each, 14.6 with four lanes). Beyond a
-// warp's 1024 elements, up to warp_row, a warp that streams; then a CTA, the larger the longer the row: what follows a row's last load --
-// joins, its numbers -- takes a CTA's time whatever its size, and the CTAs of an SM should be in different phases (16 384 rows of 3001 with
-// gradient: 128 threads 85 us, 512 152). Eight vectors in flight and half an SM's threads beat four and all of them, which leaves 32
-// registers a thread: 4096 rows of 26 000 71, 92 us. With gradient, what the CTAs of all SMs read must still be in L2 when it is read
-// again: few large ones from long_row on (4096 rows of 26 000: 256 threads 160 us, 512 178; of 32 768: 202, 182).
+// Calls as() with the kernel's shape for rows of this length.
+// Up to 1024 elements: the fewest lanes that hold a row in eight vectors each, as every lane less shares the row's numbers and shuffles
+// among more rows (131 072 rows of 125: 37 us with a warp each, 14.6 with four lanes).
+// Up to warp_row: a warp that streams. Sums: 16 384 rows of 3001 39 us, 49 by CTAs of 128; of 5000 59, 66. With gradient: 32 768 rows of
+// 1500 85 (eight vectors in flight; 90 with four), 111; of 3001 113, 85.
+// Then a CTA, the larger the longer the row: what follows a row's last load -- joins, its numbers -- takes a CTA's time whatever its
+// size, and the CTAs of an SM should be in different phases. With gradient, 128, 256 and 512 threads: 16 384 rows of 5000 124, 132, 163;
+// 8192 of 8000 111, 97, 107; 4096 of 12 000 93, 82, 82.
+// Beyond 12 000 eight vectors in flight on half an SM's threads instead of four on all of them, which leaves those 32 registers each:
+// 4096 rows of 16 384 46 and 98 us (sums, with gradient), 50 and 102; but 8192 of 9000 64 and 124, 61 and 115.
+// With gradient, what the CTAs of all SMs read must still be in L2 when it is read again, so from long_row on they are few and large:
+// 4096 rows of 26 000 160 us with 256 threads, 178 with 512; of 32 768 202, 182.
 template <int WARP_NV, typename As>
 auto by_length(const RowShape& w, int warp_row, int long_row, As as) {
   if (w.fits(1, 4)) return as(Lanes<256, 1, 4, true>{});

@@ -92,7 +92,7 @@ embed_forward_kernel(Ids ids, const float* table, float* __restrict__ y, long lo
 // ---- sort. Up to kSmallSort pairs: every pair's place is the number of pairs in front of it, counted by comparison with all. More: tiles
 // of consecutive keys, one CTA each; a pass is the count of every digit in every tile, then the scatter, whose CTAs add up the counts in
 // front of their own.
-constexpr int kSmallSort = 8192;
+constexpr int kSmallSort = 6000;
 constexpr int kSortThreads = 512;
 constexpr int kDigits = 512;              // of nine bits
 constexpr int kTiles = 148;
@@ -106,12 +106,14 @@ __device__ __forceinline__ uint2 pair_at(const Keys& k, long long t) {
   return k.pairs ? ld_plain(k.pairs + t) : make_uint2(key_of(k.ids, t), (unsigned)t);
 }
 
-// 32 pairs to a CTA, a lane each; a warp counts in its eighth of the keys, four to a load that all lanes share. An equal key
-// counts where its position is lower. One launch against four: 300 pairs 4 us, 7007 15, where the passes take some 25.
-__global__ void __launch_bounds__(kThreads) sort_small_kernel(Ids ids, uint2* __restrict__ out, int N) {
+// 32 pairs to a CTA, a lane each; a warp counts in its share of the keys, four to a load that all lanes share. An equal key
+// counts where its position is lower. One launch against four: the gradient of
+// 300 tokens of 100 values takes 11.4 us so and 17 by the passes, of 4000 22.8 and 28, of 8000 33 and 31.
+constexpr int kRankThreads = 512;
+__global__ void __launch_bounds__(kRankThreads) sort_small_kernel(Ids ids, uint2* __restrict__ out, int N) {
   chain_wait();
   chain_next();
-  constexpr int kWarps = kThreads / 32;
+  constexpr int kWarps = kRankThreads / 32;
   __shared__ __align__(16) unsigned keys[kSmallSort];
   __shared__ int counted[kWarps][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i0 = blockIdx.x * 32, i = i0 + lane;
@@ -120,21 +122,23 @@ __global__ void __launch_bounds__(kThreads) sort_small_kernel(Ids ids, uint2* __
 #pragma unroll 8
   for (int j = j0 + lane; j < end; j += 32) keys[j] = j < j1 ? key_of(ids, j) : 0xffffffffu;
   __syncwarp();
-  int n = 0;
+  int n = 0, m = 0;
   // keys in front of the CTA's own, its own, and those behind (i0 and the shares are multiples of four)
   const int own0 = min(max(i0, j0), end), own1 = min(max(i0 + 32, j0), end);
 #pragma unroll 8
   for (int j = j0; j < own0; j += 4) {
     const uint4 q = *(const uint4*)&keys[j];
-    n += (q.x <= key) + (q.y <= key) + (q.z <= key) + (q.w <= key);
+    n += (q.x <= key) + (q.y <= key);
+    m += (q.z <= key) + (q.w <= key);
   }
   for (int j = own0; j < own1; ++j) n += keys[j] < key || (keys[j] == key && j < i);
 #pragma unroll 8
   for (int j = own1; j < end; j += 4) {
     const uint4 q = *(const uint4*)&keys[j];
-    n += (q.x < key) + (q.y < key) + (q.z < key) + (q.w < key);
+    n += (q.x < key) + (q.y < key);
+    m += (q.z < key) + (q.w < key);
   }
-  counted[warp][lane] = n;
+  counted[warp][lane] = n + m;
   __syncthreads();
   if (warp == 0 && i < N) {
     int place = 0;
@@ -440,6 +444,7 @@ SortPlan sort_plan(long long N, long long V) {
 }
 
 // Places per tile of the sums: eight, one round of loads, or as many as make kSumTiles tiles; narrow rows, a few lanes each, take more tiles
+// (131 072 tokens of 4 values 54 us, 63 with as many as wide ones; of 64 52, 58)
 int sum_tile(long long N, int D) {
   int lanes = 1;
   while (lanes < 32 && lanes < (D % 4 == 0 ? D / 4 : D)) lanes *= 2;
@@ -509,7 +514,7 @@ int launch_sums(RunSums q, cudaStream_t s) {
   while (q.L < 32 && q.L < q.vectors) q.L *= 2;
   q.slices = (q.vectors + q.L - 1) / q.L;
   q.sum_ctas = (int)(((long long)q.tiles * q.slices * q.L + kThreads - 1) / kThreads);
-  // a warp zeroes up to 32 KB: 32 rows, or a share of them
+  // a warp zeroes up to 32 KB: 32 rows, or a share of them (8 KB: 131 072 tokens of 512 145 us instead of 131, each share looks its rows up)
   q.zero_shares = (q.D + 255) / 256;
   const long long zero_ctas = ((q.V + 31) / 32 * q.zero_shares + kThreads / 32 - 1) / (kThreads / 32);
   (void)launch_chained(embed_run_sums_kernel<VEC>, (unsigned)(q.sum_ctas + zero_ctas), kThreads, 0, s, 0, q);
@@ -609,7 +614,7 @@ int snntc_embedding_backward(const void* ids, int id_bytes, const void* sorted, 
   if (sorted) {
     pairs = (uint2*)sorted;
   } else if (N <= kSmallSort) {
-    (void)launch_chained(sort_small_kernel, (unsigned)((N + 31) / 32), kThreads, 0, s, 0, in, pairs, (int)N);
+    (void)launch_chained(sort_small_kernel, (unsigned)((N + 31) / 32), kRankThreads, 0, s, 0, in, pairs, (int)N);
     if (const int rc = done()) return rc;
   } else if (const int rc = launch_sort(in, N, V, pairs, (uint2*)(base + w.sort.other), (int*)(base + w.sort.counts), false, s)) {
     return rc;
