@@ -34,29 +34,82 @@ __device__ __forceinline__ unsigned key_of(const Ids& ids, long long t) {
 
 __device__ __forceinline__ float value_of(float e, float scale, int spikes) { return spikes ? expf(scale * e) : scale * e; }
 
-// ---- vectors of VEC floats: 4 where rows and pointers allow it, else 1
-template <int VEC> struct Vec;
-template <> struct Vec<1> {
-  float v[1];
-  static __device__ __forceinline__ Vec load(const float* p) { return {{ld_plain(p)}}; }
-  static __device__ __forceinline__ Vec load_once(const float* p) { return {{ld_stream(p)}}; }
-  __device__ __forceinline__ void store(float* p) const { *p = v[0]; }
-  __device__ __forceinline__ void store_once(float* p) const { __stcs(p, v[0]); }
+// ---- what a lane takes of a row of D as its c-th part: FOUR, four floats loaded as one, where rows and pointers lie on 16 bytes; else ONE,
+// or in long rows APART, four that are a warp's width apart, so that the loads of neighbouring lanes are of neighbours and as much is in
+// flight (lookup and gradient of 65 536 tokens of 511 values: ONE 55 and 121 us, APART 43 and 108; 131 072 of 129: 35 and 73, 39 and 79).
+enum Kind { ONE, FOUR, APART };
+constexpr int kApart = 256;              // from this length on
+__host__ __device__ constexpr int parts_of(Kind kind, int D) { return kind == FOUR ? D / 4 : kind == ONE ? D : (D + 127) / 128 * 32; }
+
+template <Kind KIND>
+struct Part {
+  static constexpr int N = KIND == ONE ? 1 : 4;
+  float v[N];
 };
-template <> struct Vec<4> {
-  float v[4];
-  static __device__ __forceinline__ Vec of(float4 q) { return {{q.x, q.y, q.z, q.w}}; }
-  static __device__ __forceinline__ Vec load(const float* p) { return of(ld_plain((const float4*)p)); }
-  static __device__ __forceinline__ Vec load_once(const float* p) { return of(ld_stream((const float4*)p)); }
-  __device__ __forceinline__ void store(float* p) const { *(float4*)p = make_float4(v[0], v[1], v[2], v[3]); }
-  __device__ __forceinline__ void store_once(float* p) const { __stcs((float4*)p, make_float4(v[0], v[1], v[2], v[3])); }
-};
+template <Kind KIND>
+__device__ __forceinline__ Part<KIND> load_part(const float* row, int c, int D) {
+  if constexpr (KIND == ONE) {
+    return {{ld_plain(row + c)}};
+  } else if constexpr (KIND == FOUR) {
+    const float4 q = ld_plain((const float4*)row + c);
+    return {{q.x, q.y, q.z, q.w}};
+  } else {
+    Part<KIND> q = {};
+    const int at = c + (c >> 5) * 96;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (at + 32 * k < D) q.v[k] = ld_plain(row + at + 32 * k);
+    return q;
+  }
+}
+template <Kind KIND>
+__device__ __forceinline__ Part<KIND> load_part_once(const float* row, int c, int D) {
+  if constexpr (KIND == ONE) {
+    return {{ld_stream(row + c)}};
+  } else if constexpr (KIND == FOUR) {
+    const float4 q = ld_stream((const float4*)row + c);
+    return {{q.x, q.y, q.z, q.w}};
+  } else {
+    Part<KIND> q = {};
+    const int at = c + (c >> 5) * 96;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (at + 32 * k < D) q.v[k] = ld_stream(row + at + 32 * k);
+    return q;
+  }
+}
+template <Kind KIND>
+__device__ __forceinline__ void store_part(float* row, int c, int D, const Part<KIND>& q) {
+  if constexpr (KIND == ONE) {
+    row[c] = q.v[0];
+  } else if constexpr (KIND == FOUR) {
+    ((float4*)row)[c] = make_float4(q.v[0], q.v[1], q.v[2], q.v[3]);
+  } else {
+    const int at = c + (c >> 5) * 96;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (at + 32 * k < D) row[at + 32 * k] = q.v[k];
+  }
+}
+template <Kind KIND>
+__device__ __forceinline__ void store_part_once(float* row, int c, int D, const Part<KIND>& q) {
+  if constexpr (KIND == ONE) {
+    __stcs(row + c, q.v[0]);
+  } else if constexpr (KIND == FOUR) {
+    __stcs((float4*)row + c, make_float4(q.v[0], q.v[1], q.v[2], q.v[3]));
+  } else {
+    const int at = c + (c >> 5) * 96;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (at + 32 * k < D) __stcs(row + at + 32 * k, q.v[k]);
+  }
+}
 
 constexpr int kThreads = 256;
-// L lanes to a row of `vectors` vectors. A lane has AHEAD rows in flight -- an id and then its row are two loads one behind the other -- and
-// of each COLUMNS vectors, so that what a row's read opens in memory is read at once. us, (AHEAD, COLUMNS) = (4, 1), (2, 2), (1, 4): 131 072
-// rows of 512 values 65.6, 59.6, 61.7; 10^6 of 64 67.8, 92, 123 (one vector a lane: the second is never there).
-template <int VEC, int AHEAD, int COLUMNS>
+// L lanes to a row of `vectors` parts. A lane has AHEAD rows in flight -- an id and then its row are two loads one behind the other -- and
+// of each COLUMNS parts, so that what a row's read opens in memory is read at once. us, (AHEAD, COLUMNS) = (4, 1), (2, 2), (1, 4): 131 072
+// rows of 512 values 65.6, 59.6, 61.7; 10^6 of 64 67.8, 92, 123 (one part a lane: the second is never there).
+template <Kind KIND, int AHEAD, int COLUMNS>
 __global__ void __launch_bounds__(kThreads)
 embed_forward_kernel(Ids ids, const float* table, float* __restrict__ y, long long N, int D, int vectors, int L, float scale, int spikes,
                      float no_spike) {
@@ -68,12 +121,12 @@ embed_forward_kernel(Ids ids, const float* table, float* __restrict__ y, long lo
 #pragma unroll
   for (int k = 0; k < AHEAD; ++k) key[k] = t0 + k * rows < N ? key_of(ids, t0 + k * rows) : (unsigned)ids.V;
   for (int c0 = gl; c0 < vectors; c0 += COLUMNS * L) {
-    Vec<VEC> q[AHEAD][COLUMNS];
+    Part<KIND> q[AHEAD][COLUMNS];
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
 #pragma unroll
       for (int m = 0; m < COLUMNS; ++m)
-        if (key[k] != (unsigned)ids.V && c0 + m * L < vectors) q[k][m] = Vec<VEC>::load(table + (long long)key[k] * D + (c0 + m * L) * VEC);
+        if (key[k] != (unsigned)ids.V && c0 + m * L < vectors) q[k][m] = load_part<KIND>(table + (long long)key[k] * D, c0 + m * L, D);
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
       if (t0 + k * rows >= N) break;
@@ -82,8 +135,8 @@ embed_forward_kernel(Ids ids, const float* table, float* __restrict__ y, long lo
       for (int m = 0; m < COLUMNS; ++m) {
         if (c0 + m * L >= vectors) break;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) q[k][m].v[j] = token ? value_of(q[k][m].v[j], scale, spikes) : no_spike;
-        q[k][m].store_once(y + (t0 + k * rows) * D + (c0 + m * L) * VEC);
+        for (int j = 0; j < Part<KIND>::N; ++j) q[k][m].v[j] = token ? value_of(q[k][m].v[j], scale, spikes) : no_spike;
+        store_part_once<KIND>(y + (t0 + k * rows) * D, c0 + m * L, D, q[k][m]);
       }
     }
   }
@@ -235,7 +288,7 @@ sort_scatter_kernel(Keys keys, const int* counts, uint2* __restrict__ out, long 
 
 // ---- sums of runs of equal keys. What bounds them is memory: g read once, the table's gradient written once (131 072 tokens of 512
 // values on as many rows: 537 MB in 92 us, 5.8 TB/s, behind 26 us of sort and before 8 us of joins).
-// The sorted pairs are cut into tiles of M; a group of L lanes takes a tile and L vectors of the rows, kTermsAhead rows of g in flight.
+// The sorted pairs are cut into tiles of M; a group of L lanes takes a tile and L parts of the rows, kTermsAhead rows of g in flight.
 // Runs inside a tile are done there and then; of one that crosses a border the first tile leaves its part in `tail`, the others theirs in
 // `head`, and the joining kernel adds those in order. So a token that every second place holds is summed by as many CTAs as its share,
 // and the order of summation depends on the sizes alone. (One CTA for each run: 8.3 ms, most of it the most frequent token's.)
@@ -254,18 +307,18 @@ struct RunSums {
   int spikes;
 };
 
-template <int VEC>
-__device__ __forceinline__ void write_row(const RunSums& q, unsigned key, int c, Vec<VEC> sum) {
-  const long long at = (long long)key * q.D + (long long)c * VEC;
+template <Kind KIND>
+__device__ __forceinline__ void write_row(const RunSums& q, unsigned key, int c, Part<KIND> sum) {
+  const long long row = (long long)key * q.D;
   if (q.spikes) {
-    const Vec<VEC> e = Vec<VEC>::load(q.table + at);
+    const Part<KIND> e = load_part<KIND>(q.table + row, c, q.D);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) sum.v[j] *= q.scale * expf(q.scale * e.v[j]);
+    for (int j = 0; j < Part<KIND>::N; ++j) sum.v[j] *= q.scale * expf(q.scale * e.v[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) sum.v[j] *= q.scale;
+    for (int j = 0; j < Part<KIND>::N; ++j) sum.v[j] *= q.scale;
   }
-  sum.store(q.dtable + at);
+  store_part<KIND>(q.dtable + row, c, q.D, sum);
 }
 
 __device__ void zero_rows(const RunSums& q) {
@@ -304,7 +357,7 @@ __device__ void zero_rows(const RunSums& q) {
   }
 }
 
-template <int VEC>
+template <Kind KIND>
 __global__ void __launch_bounds__(kThreads) embed_run_sums_kernel(RunSums q) {
   chain_wait();
   chain_next();
@@ -317,50 +370,50 @@ __global__ void __launch_bounds__(kThreads) embed_run_sums_kernel(RunSums q) {
   unsigned key = ld_plain(&q.pairs[i0].x);
   const unsigned after = i1 < q.N ? ld_plain(&q.pairs[i1].x) : none;
   bool from_before = i0 > 0 && ld_plain(&q.pairs[i0 - 1].x) == key;
-  Vec<VEC> sum = {};
+  Part<KIND> sum = {};
   for (long long i = i0; i < i1; i += kTermsAhead) {
     uint2 p[kTermsAhead];
-    Vec<VEC> x[kTermsAhead];
+    Part<KIND> x[kTermsAhead];
 #pragma unroll
     for (int k = 0; k < kTermsAhead; ++k) p[k] = i + k < i1 ? ld_plain(q.pairs + i + k) : make_uint2(none, 0);
 #pragma unroll
     for (int k = 0; k < kTermsAhead; ++k)
-      if (p[k].x < q.V) x[k] = Vec<VEC>::load_once(q.g + (long long)p[k].y * q.D + c * VEC);
+      if (p[k].x < q.V) x[k] = load_part_once<KIND>(q.g + (long long)p[k].y * q.D, c, q.D);
 #pragma unroll
     for (int k = 0; k < kTermsAhead; ++k) {
       if (p[k].x == none) break;
       if (p[k].x != key) {
-        if (from_before) sum.store(q.head + (long long)tile * q.D + c * VEC);
-        else write_row<VEC>(q, key, c, sum);
+        if (from_before) store_part<KIND>(q.head + (long long)tile * q.D, c, q.D, sum);
+        else write_row<KIND>(q, key, c, sum);
         key = p[k].x;
         from_before = false;
         sum = {};
       }
       if (key >= q.V) return;             // what is no token sorts behind all tokens
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) sum.v[j] += x[k].v[j];
+      for (int j = 0; j < Part<KIND>::N; ++j) sum.v[j] += x[k].v[j];
     }
   }
-  if (from_before) sum.store(q.head + (long long)tile * q.D + c * VEC);
-  else if (key == after) sum.store(q.tail + (long long)tile * q.D + c * VEC);
-  else write_row<VEC>(q, key, c, sum);
+  if (from_before) store_part<KIND>(q.head + (long long)tile * q.D, c, q.D, sum);
+  else if (key == after) store_part<KIND>(q.tail + (long long)tile * q.D, c, q.D, sum);
+  else write_row<KIND>(q, key, c, sum);
 }
 
-// Runs that go on behind the tile in which they begin: a warp looks at a tile and 32 vectors, adds a run of a few tiles itself and leaves
+// Runs that go on behind the tile in which they begin: a warp looks at a tile and 32 parts, adds a run of a few tiles itself and leaves
 // a longer one to all warps of its CTA, an eighth of the tiles each.
-template <int VEC>
+template <Kind KIND>
 __global__ void __launch_bounds__(kThreads) embed_join_kernel(RunSums q) {
   chain_wait();
   chain_next();
   constexpr int kWarps = kThreads / 32, kFew = 8;
-  __shared__ Vec<VEC> part[kWarps][32];
+  __shared__ Part<KIND> part[kWarps][32];
   __shared__ int last_tile[kWarps];        // of a run that is left to all; 0: none (a run's last tile is behind its first)
   const int columns = (q.vectors + 31) / 32, tile0 = (int)(blockIdx.x / columns) * kWarps;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = (int)(blockIdx.x % columns) * 32 + lane;
-  const auto head_of = [&](int t) { return Vec<VEC>::load(q.head + (long long)t * q.D + c * VEC); };
-  const auto add = [](Vec<VEC>& sum, const Vec<VEC>& x) {
+  const auto head_of = [&](int t) { return load_part<KIND>(q.head + (long long)t * q.D, c, q.D); };
+  const auto add = [](Part<KIND>& sum, const Part<KIND>& x) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) sum.v[j] += x.v[j];
+    for (int j = 0; j < Part<KIND>::N; ++j) sum.v[j] += x.v[j];
   };
   {
     const int tile = tile0 + warp;
@@ -381,10 +434,10 @@ __global__ void __launch_bounds__(kThreads) embed_join_kernel(RunSums q) {
     }
     if (last && last - tile <= kFew) {
       if (c < q.vectors) {
-        Vec<VEC> sum = Vec<VEC>::load(q.tail + (long long)tile * q.D + c * VEC);
+        Part<KIND> sum = load_part<KIND>(q.tail + (long long)tile * q.D, c, q.D);
 #pragma unroll 4
         for (int t = tile + 1; t <= last; ++t) add(sum, head_of(t));
-        write_row<VEC>(q, key, c, sum);
+        write_row<KIND>(q, key, c, sum);
       }
       last = 0;
     }
@@ -394,16 +447,16 @@ __global__ void __launch_bounds__(kThreads) embed_join_kernel(RunSums q) {
   for (int k = 0; k < kWarps; ++k) {
     const int last = last_tile[k], tile = tile0 + k;
     if (last == 0) continue;
-    Vec<VEC> sum = {};
+    Part<KIND> sum = {};
     if (c < q.vectors)
 #pragma unroll 8
       for (int t = tile + 1 + warp; t <= last; t += kWarps) add(sum, head_of(t));
     part[warp][lane] = sum;
     __syncthreads();
     if (warp == 0 && c < q.vectors) {
-      sum = Vec<VEC>::load(q.tail + (long long)tile * q.D + c * VEC);
+      sum = load_part<KIND>(q.tail + (long long)tile * q.D, c, q.D);
       for (int w = 0; w < kWarps; ++w) add(sum, part[w][lane]);
-      write_row<VEC>(q, ld_plain(&q.pairs[(long long)tile * q.M + q.M - 1].x), c, sum);
+      write_row<KIND>(q, ld_plain(&q.pairs[(long long)tile * q.M + q.M - 1].x), c, sum);
     }
     __syncthreads();
   }
@@ -447,7 +500,7 @@ SortPlan sort_plan(long long N, long long V) {
 // (131 072 tokens of 4 values 54 us, 63 with as many as wide ones; of 64 52, 58)
 int sum_tile(long long N, int D) {
   int lanes = 1;
-  while (lanes < 32 && lanes < (D % 4 == 0 ? D / 4 : D)) lanes *= 2;
+  while (lanes < 32 && lanes < parts_of(D % 4 == 0 ? FOUR : D >= kApart ? APART : ONE, D)) lanes *= 2;
   const long long tiles = (long long)kSumTiles * (lanes < 4 ? 8 : 32 / lanes), m = (N + tiles - 1) / tiles;
   return (int)((m + kTermsAhead - 1) / kTermsAhead * kTermsAhead);
 }
@@ -507,9 +560,9 @@ int launch_sort(const Ids& ids, long long N, long long V, uint2* sorted, uint2* 
   return SNNTC_OK;
 }
 
-template <int VEC>
+template <Kind KIND>
 int launch_sums(RunSums q, cudaStream_t s) {
-  q.vectors = q.D / VEC;
+  q.vectors = parts_of(KIND, q.D);
   q.L = 1;
   while (q.L < 32 && q.L < q.vectors) q.L *= 2;
   q.slices = (q.vectors + q.L - 1) / q.L;
@@ -517,10 +570,10 @@ int launch_sums(RunSums q, cudaStream_t s) {
   // a warp zeroes up to 32 KB: 32 rows, or a share of them (8 KB: 131 072 tokens of 512 145 us instead of 131, each share looks its rows up)
   q.zero_shares = (q.D + 255) / 256;
   const long long zero_ctas = ((q.V + 31) / 32 * q.zero_shares + kThreads / 32 - 1) / (kThreads / 32);
-  (void)launch_chained(embed_run_sums_kernel<VEC>, (unsigned)(q.sum_ctas + zero_ctas), kThreads, 0, s, 0, q);
+  (void)launch_chained(embed_run_sums_kernel<KIND>, (unsigned)(q.sum_ctas + zero_ctas), kThreads, 0, s, 0, q);
   if (const int rc = done()) return rc;
   if (q.tiles == 1) return SNNTC_OK;
-  (void)launch_chained(embed_join_kernel<VEC>, (unsigned)((q.tiles + 7) / 8 * ((q.vectors + 31) / 32)), kThreads, 0, s, 0, q);
+  (void)launch_chained(embed_join_kernel<KIND>, (unsigned)((q.tiles + 7) / 8 * ((q.vectors + 31) / 32)), kThreads, 0, s, 0, q);
   return done();
 }
 
@@ -529,8 +582,8 @@ int launch_sums(RunSums q, cudaStream_t s) {
 bool sorts_beside(long long N, int D) { return N > kSmallSort && N * D >= (4LL << 20); }
 
 int launch_lookup(const Ids& in, const float* table, float* y, long long N, int D, float scale, int spikes, float no_spike, cudaStream_t s) {
-  const bool four = by_four(D, table, y, nullptr);
-  const int vectors = four ? D / 4 : D;
+  const Kind kind = by_four(D, table, y, nullptr) ? FOUR : D >= kApart ? APART : ONE;
+  const int vectors = parts_of(kind, D);
   int L = 1;                                // lanes to a row: up to a warp
   while (L < 32 && L < vectors) L *= 2;
   const auto launch = [&](auto kernel, int ahead) {
@@ -538,8 +591,10 @@ int launch_lookup(const Ids& in, const float* table, float* y, long long N, int 
     (void)launch_chained(kernel, (unsigned)((N + rows - 1) / rows), kThreads, 0, s, 0, in, table, y, N, D, vectors, L, scale, spikes, no_spike);
     return done();
   };
-  if (vectors <= 32) return four ? launch(embed_forward_kernel<4, 4, 1>, 4) : launch(embed_forward_kernel<1, 4, 1>, 4);
-  return four ? launch(embed_forward_kernel<4, 2, 2>, 2) : launch(embed_forward_kernel<1, 2, 2>, 2);
+  if (vectors <= 32) return kind == FOUR ? launch(embed_forward_kernel<FOUR, 4, 1>, 4) : launch(embed_forward_kernel<ONE, 4, 1>, 4);
+  return kind == FOUR  ? launch(embed_forward_kernel<FOUR, 2, 2>, 2)
+         : kind == ONE ? launch(embed_forward_kernel<ONE, 2, 2>, 2)
+                       : launch(embed_forward_kernel<APART, 2, 2>, 2);
 }
 
 }  // namespace
@@ -633,7 +688,8 @@ int snntc_embedding_backward(const void* ids, int id_bytes, const void* sorted, 
   q.tiles = (int)((N + q.M - 1) / q.M);
   q.scale = scale;
   q.spikes = spikes;
-  return by_four(D, g, dtable, spikes ? table : nullptr) ? launch_sums<4>(q, s) : launch_sums<1>(q, s);
+  if (by_four(D, g, dtable, spikes ? table : nullptr)) return launch_sums<FOUR>(q, s);
+  return D >= kApart ? launch_sums<APART>(q, s) : launch_sums<ONE>(q, s);
 }
 
 }  // extern "C"
