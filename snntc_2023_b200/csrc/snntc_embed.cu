@@ -109,6 +109,7 @@ constexpr int kThreads = 256;
 // L lanes to a row of `vectors` parts. A lane has AHEAD rows in flight -- an id and then its row are two loads one behind the other -- and
 // of each COLUMNS parts, so that what a row's read opens in memory is read at once. us, (AHEAD, COLUMNS) = (4, 1), (2, 2), (1, 4): 131 072
 // rows of 512 values 65.6, 59.6, 61.7; 10^6 of 64 67.8, 92, 123 (one part a lane: the second is never there).
+// Of single places (4, 4): 131 072 rows of 201 41 us, 45 with (2, 2).
 template <Kind KIND, int AHEAD, int COLUMNS>
 __global__ void __launch_bounds__(kThreads)
 embed_forward_kernel(Ids ids, const float* table, float* __restrict__ y, long long N, int D, int vectors, int L, float scale, int spikes,
@@ -145,7 +146,7 @@ embed_forward_kernel(Ids ids, const float* table, float* __restrict__ y, long lo
 // ---- sort. Up to kSmallSort pairs: every pair's place is the number of pairs in front of it, counted by comparison with all. More: tiles
 // of consecutive keys, one CTA each; a pass is the count of every digit in every tile, then the scatter, whose CTAs add up the counts in
 // front of their own.
-constexpr int kSmallSort = 6000;
+constexpr int kSmallSort = 8192;
 constexpr int kSortThreads = 512;
 constexpr int kDigits = 512;              // of nine bits
 constexpr int kTiles = 148;
@@ -159,9 +160,9 @@ __device__ __forceinline__ uint2 pair_at(const Keys& k, long long t) {
   return k.pairs ? ld_plain(k.pairs + t) : make_uint2(key_of(k.ids, t), (unsigned)t);
 }
 
-// 32 pairs to a CTA, a lane each; a warp counts in its share of the keys, four to a load that all lanes share. An equal key
-// counts where its position is lower. One launch against four: the gradient of
-// 300 tokens of 100 values takes 11.4 us so and 17 by the passes, of 4000 22.8 and 28, of 8000 33 and 31.
+// 32 pairs to a CTA, a lane each; a warp counts in its share of the keys, four to a load that all lanes share. An equal key counts
+// where its position is lower. One launch against four: the gradient of 300 tokens of 100 values takes 11.4 us so and 17 by the passes, of
+// 4000 22.8 and 28, of 8000 33 and 31 -- but three launches less for the host, whose time that is at these sizes (a step of 7007 60, 66).
 constexpr int kRankThreads = 512;
 __global__ void __launch_bounds__(kRankThreads) sort_small_kernel(Ids ids, uint2* __restrict__ out, int N) {
   chain_wait();
@@ -593,7 +594,7 @@ int launch_lookup(const Ids& in, const float* table, float* y, long long N, int 
   };
   if (vectors <= 32) return kind == FOUR ? launch(embed_forward_kernel<FOUR, 4, 1>, 4) : launch(embed_forward_kernel<ONE, 4, 1>, 4);
   return kind == FOUR  ? launch(embed_forward_kernel<FOUR, 2, 2>, 2)
-         : kind == ONE ? launch(embed_forward_kernel<ONE, 2, 2>, 2)
+         : kind == ONE ? launch(embed_forward_kernel<ONE, 4, 4>, 4)
                        : launch(embed_forward_kernel<APART, 2, 2>, 2);
 }
 

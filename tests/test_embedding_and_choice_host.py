@@ -24,7 +24,7 @@ def test_status_codes_of_the_embedding():
     assert bwd(N=-1) == bwd(V=0) == bwd(D=0) == -2
     assert bwd(ws=0) == bwd(ws=FAKE + 8) == bwd(n=size(5, 7, 3) - 1) == -5
     kept, scratch = lib.snntc_embedding_sorted_bytes, lib.snntc_embedding_sort_workspace_bytes
-    assert kept(0, 9) == kept(6000, 9999) == scratch(6000, 9999) == kept(6001, 9) == 0   # a short lookup: the backward sorts
+    assert kept(0, 9) == kept(8192, 9999) == scratch(8192, 9999) == kept(8193, 9) == 0   # a short lookup: the backward sorts
     assert kept(8193, 512) == 8193 * 8 and scratch(8193, 512) > 8193 * 8
     both = lambda ids=FAKE, table=FAKE, y=FAKE, out=FAKE, N=9000, ws=FAKE, n=1 << 40: lib.snntc_embedding_forward_sort(  # noqa: E731
         ids, 8, table, y, N, 7, 512, 1.0, 0, -1, 1e5, out, ws, n, 0)

@@ -49,7 +49,7 @@ def _check(ids, table, up, y, grad, scale, spikes, padding=None, no_spike=1e5):
 
 SIZES = [(1, 1, 1), (1, 10007, 784), (2, 2, 3), (31, 7, 4), (32, 1, 33), (33, 300, 128), (257, 255, 129), (257, 256, 64), (300, 257, 100),
          (1000, 65536, 12), (4097, 1000, 100), (5000, 3, 257), (7007, 50021, 129), (20000, 65535, 36), (40000, 131072, 8), (70001, 90, 16),
-         (3, 100, 5000), (65536, 1 << 20, 4), (40, 3, 2_100_001), (8192, 40, 7), (8193, 40, 8), (8200, 600, 31), (303_105, 513, 3), (150_000, 262_144, 2), (8193, 1000, 512), (6000, 777, 20), (6001, 777, 20), (6001, 500, 701), (8500, 300_000, 515),
+         (3, 100, 5000), (65536, 1 << 20, 4), (40, 3, 2_100_001), (8192, 40, 7), (8193, 40, 8), (8200, 600, 31), (303_105, 513, 3), (150_000, 262_144, 2), (8193, 1000, 512), (8192, 777, 20), (8193, 777, 20), (8193, 500, 701), (8500, 300_000, 515),
          (40_000, 9, 128)]
 
 
