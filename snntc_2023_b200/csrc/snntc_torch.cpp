@@ -17,6 +17,8 @@
 #include <cmath>
 #include <cstring>
 #include <mutex>
+#include <unordered_set>
+#include <vector>
 
 #include "../../include/snntc_b200.h"
 
@@ -547,10 +549,12 @@ Tensor constraint_cost(const std::vector<Tensor>& weights, double K, double K2) 
 
 // ------------------------------------------------------------------------------------------------ embedding, losses on choices
 // The nodes below compute gradients by kernels that nothing differentiates: asked for a graph of the gradient they refuse, instead
-// of handing out one that is a constant. And a leaf whose gradient accumulator lives on another stream -- an eager graph of the
-// same leaf is still alive -- would draw that stream into a capture under way, which ends the process: refused as well, before
-// autograd gets there.
+// of handing out one that is a constant. And a leaf whose gradient accumulator lives on the default stream -- a graph of the same
+// leaf that was built there is still alive -- would draw that stream, which nothing can capture, into a capture under way, which ends
+// the process: refused as well, before autograd gets there, for all leaves that this pass goes on to. (Accumulators of other streams
+// join the capture and are joined by it.)
 void check_backward(const Tensor& on, const char* what) {
+  using torch::autograd::Node;
   if (at::GradMode::is_enabled()) throw SnntcFailure(std::string(what) + ": the gradient cannot be differentiated again (create_graph)");
   const auto current = at::cuda::getCurrentCUDAStream(on.get_device());
   cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
@@ -559,13 +563,28 @@ void check_backward(const Tensor& on, const char* what) {
     return;
   }
   if (capturing == cudaStreamCaptureStatusNone) return;
-  for (const torch::autograd::Edge& edge : torch::autograd::get_current_node()->next_edges()) {
-    auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get());
-    if (leaf == nullptr) continue;
-    const auto stream = leaf->stream();
-    if (stream.has_value() && *stream != current.unwrap())
-      throw SnntcFailure(std::string(what) + ": a backward pass is being captured while a graph of the same leaf that was built on "
-                         "another stream is alive; release that graph (its outputs) before the capture");
+  const auto* wanted = torch::autograd::get_current_graph_task_exec_info();     // empty: all nodes run
+  const auto foreign = at::cuda::getDefaultCUDAStream(on.get_device()).unwrap();
+  std::vector<Node*> todo = {torch::autograd::get_current_node().get()};
+  std::unordered_set<Node*> seen(todo.begin(), todo.end());
+  while (!todo.empty()) {
+    Node* node = todo.back();
+    todo.pop_back();
+    for (const torch::autograd::Edge& edge : node->next_edges()) {
+      Node* next = edge.function.get();
+      if (next == nullptr || !seen.insert(next).second) continue;
+      if (wanted && !wanted->empty()) {
+        const auto it = wanted->find(next);
+        if (it == wanted->end() || !it->second.should_execute()) continue;
+      }
+      todo.push_back(next);
+      auto* leaf = dynamic_cast<torch::autograd::AccumulateGrad*>(next);
+      if (leaf == nullptr) continue;
+      const auto stream = leaf->stream();
+      if (stream.has_value() && *stream == foreign)
+        throw SnntcFailure(std::string(what) + ": a backward pass is being captured while a graph of the same leaf that was built on "
+                           "the default stream is alive; release that graph (its outputs) before the capture");
+    }
   }
 }
 

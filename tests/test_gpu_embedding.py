@@ -325,3 +325,27 @@ def test_a_capture_beside_a_live_eager_graph_is_refused():
     torch.cuda.synchronize()
     alive.backward(up)                               # the eager graph is as it was
     _check(ids, table, up, alive.detach(), w.grad, 1.0, False)
+
+
+def test_a_capture_beside_a_live_graph_of_a_side_stream():
+    """The usual warm-up: on a side stream, its last graph still alive when the capture begins."""
+    import torch
+    from snntc_2023_b200 import ops
+    ids, table, up = _case(300, 20, 8, 3)
+    w = table.clone().requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = ops.snn_embedding(ids, w)
+        alive.backward(up)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    w.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.snn_embedding(ids, w)
+        y.backward(up)
+    ids.copy_(ids.flip(0))
+    graph.replay()
+    torch.cuda.synchronize()
+    _check(ids, table, up, y.detach(), w.grad, 1.0, False)

@@ -109,3 +109,29 @@ def test_texts_through_a_convolution():
         cut = net.layers[1](net.layers[0](short))[:, :, :4]
         whole = net.layers[1](net.layers[0](short[:, :, :5]))[:, :, :4]
     assert torch.equal(cut, whole)                                # fields that do not reach the padding see none of it
+
+
+def test_a_capture_beside_a_live_eager_network_is_refused():
+    """The loss says so for the leaves behind it, too, not only for its own; and only where the pass gets to them."""
+    import torch
+    from snntc_2023_b200 import train
+    w = torch.randn(6, 5, device="cuda").requires_grad_(True)
+    act = torch.tensor([0, 1, -1, 4], device="cuda")
+    x, old, adv = torch.randn(4, 6, device="cuda"), torch.full((4,), -1.6, device="cuda"), torch.ones(4, device="cuda")
+    alive = train.policy_loss((x @ w).exp(), act, old, adv)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            train.policy_loss((x @ w).exp(), act, old, adv).backward()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = (x @ w).exp()
+        (dout,) = torch.autograd.grad(train.policy_loss(out, act, old, adv), out)
+    graph.replay()
+    leaf = (x @ w).exp().detach().requires_grad_(True)
+    train.policy_loss(leaf, act, old, adv).backward()
+    torch.cuda.synchronize()
+    assert torch.equal(dout, leaf.grad)
+    alive.backward()
+    assert w.grad.isfinite().all()
