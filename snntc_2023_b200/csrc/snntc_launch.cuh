@@ -99,7 +99,8 @@ cudaError_t launch_chained(void (*kernel)(Params...), ChainGrid where, dim3 bloc
 }
 
 // Raises the kernel's limit of dynamic shared memory on the current device to at least `bytes`; a call into the runtime only
-// when it grows. What every kernel may have anyway (48 KB less its static arrays, which are below 16 KB everywhere) is not looked up.
+// when it grows. What every kernel may have anyway (48 KB less its static arrays, which are below 16 KB in all that ask here) is not
+// looked up.
 template <auto Kernel>
 cudaError_t allow_smem(size_t bytes) {
   if (bytes <= 32 * 1024) return cudaSuccess;

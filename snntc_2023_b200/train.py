@@ -45,8 +45,8 @@ def constraint_cost(weights, K, K2):
 
 def label_log_probs(logit, label):
     """log softmax(-logit)[label] of every row: logit [..., classes] spike values, label [...] integers; [...]. A row whose label
-    is outside the classes (-1, say) does not count: 0, and no gradient. The gradient cannot be differentiated again. Under no_grad this is what policy_loss and
-    preference_loss take as the old and the reference network's log-probabilities."""
+    is outside the classes (-1, say) does not count: 0, and no gradient. The gradient cannot be differentiated again. Under no_grad
+    this is what policy_loss and preference_loss take as the old and the reference network's log-probabilities."""
     return _lib.native().label_log_probs(_tensor(logit, "logit"), _tensor(label, "label"))
 
 
