@@ -30,6 +30,7 @@ using snntc::chain_wait;
 using snntc::launch_chained;
 using snntc::ld_plain;
 using snntc::ld_stream_at;
+using snntc::streaming;
 
 __device__ __forceinline__ bool counts(long long label, int J) { return label >= 0 && label < J; }
 
@@ -719,7 +720,7 @@ int launch_rows(const float* z, const long long* labels, const RowOut& out, cons
     constexpr int T = L::T, G = L::G;
     const unsigned grid = (unsigned)((R + T / G - 1) / (T / G));
     if (ctas) *ctas = grid;
-    (void)launch_chained(choice_rows_kernel<T, G, L::NV, L::HOLD, POLICY>, grid, T, 0, s, 0, z, labels, out, pol, R, J);
+    (void)launch_chained(choice_rows_kernel<T, G, L::NV, L::HOLD, POLICY>, streaming(grid), T, 0, s, 0, z, labels, out, pol, R, J);
     return done();
   });
 }
@@ -730,7 +731,7 @@ int launch_grad_as(const float* z, const long long* labels, const float* stats, 
   const int chunks = G == T ? (J + RowShape(z, J).slack + 4 * T * NV - 1) / (4 * T * NV) : 1;
   const long long grid = G == T ? R * chunks : (R + T / G - 1) / (T / G);
   if (grid > 0x7fffffffLL) return SNNTC_E_TOO_LARGE;
-  (void)launch_chained(choice_grad_kernel<T, G, NV, HOLD>, (unsigned)grid, T, 0, s, 0, z, labels, (const float2*)stats, factor, gout, dz, R, J, chunks);
+  (void)launch_chained(choice_grad_kernel<T, G, NV, HOLD>, streaming((unsigned)grid), T, 0, s, 0, z, labels, (const float2*)stats, factor, gout, dz, R, J, chunks);
   return done();
 }
 

@@ -20,6 +20,7 @@ using snntc::chain_wait;
 using snntc::launch_chained;
 using snntc::ld_plain;
 using snntc::ld_stream;
+using snntc::streaming;
 
 // Ids of 32 or 64 bits; what is no token of the table becomes V, the largest key.
 struct Ids {
@@ -589,7 +590,7 @@ int launch_lookup(const Ids& in, const float* table, float* y, long long N, int 
   while (L < 32 && L < vectors) L *= 2;
   const auto launch = [&](auto kernel, int ahead) {
     const long long rows = (long long)kThreads / L * ahead;
-    (void)launch_chained(kernel, (unsigned)((N + rows - 1) / rows), kThreads, 0, s, 0, in, table, y, N, D, vectors, L, scale, spikes, no_spike);
+    (void)launch_chained(kernel, streaming((unsigned)((N + rows - 1) / rows)), kThreads, 0, s, 0, in, table, y, N, D, vectors, L, scale, spikes, no_spike);
     return done();
   };
   if (vectors <= 32) return kind == FOUR ? launch(embed_forward_kernel<FOUR, 4, 1>, 4) : launch(embed_forward_kernel<ONE, 4, 1>, 4);
