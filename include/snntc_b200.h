@@ -217,8 +217,9 @@ SNNTC_API int snntc_sgdm_step(float* w, const float* g, float* vel, size_t n, fl
  * snntc_policy_loss  the mean over the rows that count of -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef * k with
  *                    r = exp(lp - old_logp), A = advantage, k = exp(ref_logp - lp) - (ref_logp - lp) - 1. *loss and
  *                    kl_and_clipped[2] (mean k; share of rows whose ratio was clipped) are written; 0 where no row counts.
- *                    ref_logp may be null where kl_coef is 0. dz[R,J], where it is not null, receives dloss / dz in the pass that
- *                    reads z. stats_2R and factor may be null.
+ *                    ref_logp may be null where kl_coef is 0; where it is not null then, k is formed for its mean alone. A k that
+ *                    overflows (lp far below ref_logp) is infinite, with a kl_coef the loss and the row's gradient with it.
+ *                    dz[R,J], where it is not null, receives dloss / dz in the pass that reads z. stats_2R and factor may be null.
  * snntc_scale_gradient      dz *= *gout, n elements; nothing is moved where *gout is 1.
  * snntc_preference_loss  texts 0..P-1 are preferred to texts P..2P-1: text s is rows [starts[s], starts[s+1]) (2P+1 ascending
  *                    offsets, device; they are held to [0, R]) or, where starts is null, the s-th of 2P equal parts of the rows.

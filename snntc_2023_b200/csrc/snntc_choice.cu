@@ -68,12 +68,15 @@ __device__ __forceinline__ PolicyRow policy_row(double lp, double old, double ad
   const double gain = (p.clipped ? (adv > 0 ? q.upper : q.lower) : ratio) * adv;
   p.kl = 0;
   p.slope = p.clipped ? 0 : -ratio * adv;
+  p.loss = -gain;
   if (has_ref) {
     const double away = ref - lp, e = expm1(away);
     p.kl = e - away;
-    p.slope -= q.kl_coef * e;
+    if (q.kl_coef != 0) {        // (a label that does not spike overflows e: without a weight that stays out of the loss)
+      p.slope -= q.kl_coef * e;
+      p.loss += q.kl_coef * p.kl;
+    }
   }
-  p.loss = q.kl_coef * p.kl - gain;
   return p;
 }
 

@@ -585,3 +585,57 @@ def test_a_capture_beside_a_live_eager_graph_is_refused():
     torch.cuda.synchronize()
     alive.sum().backward()
     assert z.grad.isfinite().all()
+
+
+def _beside_a_silent_label(R, J, seed):
+    """Every row counts, ratios lie at exp(+-0.1), inside the clip. In row R // 2 the label's output does not spike while others do: its
+    log-probability is near -1e5, the reference's is -3."""
+    import torch
+    z, lab = _logits(R, J, seed, ignore=0.0)
+    at = R // 2
+    z[at] = 2.0
+    z[at, lab[at]] = 1e5
+    g = torch.Generator("cuda").manual_seed(seed)
+    lp = Ref(z, lab).lp
+    old = (lp + 0.1 * torch.randn(R, device="cuda", generator=g).sign()).float()
+    adv, refp = torch.randn(R, device="cuda", generator=g), (lp + 0.1).float()
+    old[at] = lp[at].float()
+    refp[at] = -3.0
+    return z, lab, old, adv, refp, at
+
+
+SILENT = [(6, 10), (400, 60), (90, 1000), (40, 1500), (6, 5000), (4, 40000)]
+
+
+@pytest.mark.parametrize("R,J", SILENT)
+def test_a_reference_without_weight_has_no_part_in_the_loss(R, J):
+    """A KL coefficient of 0 beside a reference, for the statistics: the call without it, also where the KL term overflows."""
+    import torch
+    from snntc_2023_b200 import train
+    z, lab, old, adv, refp, at = _beside_a_silent_label(R, J, R + J)
+    results = []
+    for r in (refp, None):
+        z1 = z.clone().requires_grad_(True)
+        loss, stats = train.policy_loss(z1, lab, old, adv, ref_logp=r, with_stats=True)
+        (grad,) = torch.autograd.grad(loss, z1)
+        results.append((loss.detach(), grad, stats))
+    (loss, grad, stats), (plain, want, _) = results
+    assert loss.isfinite() and grad.isfinite().all() and torch.equal(loss, plain) and torch.equal(grad, want)
+    assert float(stats[0]) == math.inf and torch.equal(stats[1], results[1][2][1])
+
+
+@pytest.mark.parametrize("R,J", SILENT)
+def test_a_kl_term_that_overflows_stays_in_its_row(R, J):
+    """With a weight the infinite term is the formula's own: the loss is infinite, the rows beside it are as ever."""
+    import torch
+    from snntc_2023_b200 import train
+    z, lab, old, adv, refp, at = _beside_a_silent_label(R, J, R + J)
+    z1 = z.clone().requires_grad_(True)
+    loss = train.policy_loss(z1, lab, old, adv, ref_logp=refp, kl_coef=0.1)
+    (grad,) = torch.autograd.grad(loss, z1)
+    assert float(loss.detach()) == math.inf and not grad[at].isfinite().all()
+    ref = Ref(z, lab)
+    want = _policy_ref(ref, old, adv, refp, 0.2, 0.2, 0.1)
+    ref.counts[at] = False                            # (left out of what follows)
+    grad[at] = 0
+    ref.check_grad(grad, want["factor"], want["factor_tol"])
