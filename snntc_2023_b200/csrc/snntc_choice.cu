@@ -65,10 +65,10 @@ __device__ __forceinline__ PolicyRow policy_row(double lp, double old, double ad
   PolicyRow p;
   const double ratio = exp(lp - old);
   p.clipped = (adv > 0 && ratio > q.upper) || (adv < 0 && ratio < q.lower);
-  const double gain = (p.clipped ? (adv > 0 ? q.upper : q.lower) : ratio) * adv;
+  const double unclipped = adv == 0 && isinf(ratio) ? 0 : ratio * adv;      // (an advantage of 0 has no part, whatever the ratio)
   p.kl = 0;
-  p.slope = p.clipped ? 0 : -ratio * adv;
-  p.loss = -gain;
+  p.slope = p.clipped ? 0 : -unclipped;
+  p.loss = -(p.clipped ? (adv > 0 ? q.upper : q.lower) * adv : unclipped);
   if (has_ref) {
     const double away = ref - lp, e = expm1(away);
     p.kl = e - away;

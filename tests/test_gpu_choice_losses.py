@@ -639,3 +639,25 @@ def test_a_kl_term_that_overflows_stays_in_its_row(R, J):
     ref.counts[at] = False                            # (left out of what follows)
     grad[at] = 0
     ref.check_grad(grad, want["factor"], want["factor_tol"])
+
+
+@pytest.mark.parametrize("R,J", SILENT)
+def test_an_advantage_of_nothing_beside_a_ratio_that_overflows(R, J):
+    """A label that the old network gave next to nothing: its ratio overflows, and with an advantage of 0 the row has no part in the
+    loss, as with any other ratio."""
+    import torch
+    from snntc_2023_b200 import train
+    z, lab, old, adv, _, at = _beside_a_silent_label(R, J, R + J + 1)
+    z[at, lab[at]] = 1.0
+    adv[at] = 0.0
+    results = []
+    for o in (-1e5, -0.5):
+        old[at] = o
+        z1 = z.clone().requires_grad_(True)
+        loss = train.policy_loss(z1, lab, old, adv)
+        (grad,) = torch.autograd.grad(loss, z1)
+        results.append((loss.detach(), grad))
+    assert results[0][0].isfinite() and not results[0][1][at].any()
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    z[at, 0] = float("nan")                           # what is no number stays so
+    assert train.policy_loss(z, lab, old, adv).isnan()
