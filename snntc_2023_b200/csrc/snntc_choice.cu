@@ -634,7 +634,8 @@ preference_pairs_kernel(const double* lp, const long long* starts, const float* 
       if (ref) { good -= ld_plain(ref + k); bad -= ld_plain(ref + P + k); }
       const double m = beta * (good - bad);
       const double far = log1p(exp(-fabs(m)));                 // -log sigma(|m|)
-      const double term = (1 - smoothing) * (far + fmax(-m, 0.0)) + smoothing * (far + fmax(m, 0.0));
+      // (a margin is infinite where an output at +inf rules a text's label out: a side without weight has no part then, either)
+      const double term = (smoothing < 1 ? (1 - smoothing) * (far + fmax(-m, 0.0)) : 0.0) + (smoothing > 0 ? smoothing * (far + fmax(m, 0.0)) : 0.0);
       if (FEW) total.x += term;
       else terms[k] = term;
       margins[k] = (float)m;

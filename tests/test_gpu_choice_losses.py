@@ -661,3 +661,26 @@ def test_an_advantage_of_nothing_beside_a_ratio_that_overflows(R, J):
     assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
     z[at, 0] = float("nan")                           # what is no number stays so
     assert train.policy_loss(z, lab, old, adv).isnan()
+
+
+@pytest.mark.parametrize("P", [2, 20])
+@pytest.mark.parametrize("smoothing", [0.0, 1.0])
+def test_a_margin_without_bounds_beside_a_smoothing_of_nothing(P, smoothing):
+    """A text with a label that its network rules out (an output at +inf) has an infinite margin. Where that is the side which the
+    loss wants, the pair's loss is 0, as its limit is: -log sigma(inf), and nothing of the other side's."""
+    import torch
+    from snntc_2023_b200 import train
+    z, lab = _logits(6 * P, 12, P, ignore=0.0)
+    starts = torch.arange(0, 6 * P + 1, 3, device="cuda")
+    refp = train.label_log_probs(z, lab).view(2 * P, 3).sum(1)            # margins near 0 elsewhere
+    row = 3 * P + 1 if smoothing == 0 else 1                              # of the rejected text of pair 0, or of the preferred one
+    z[row, lab[row]] = float("inf")
+    z1 = z.clone().requires_grad_(True)
+    loss, m = train.preference_loss(z1, lab, starts, ref_logp=refp, label_smoothing=smoothing, with_margins=True)
+    (grad,) = torch.autograd.grad(loss, z1)
+    assert float(m[0]) == (math.inf if smoothing == 0 else -math.inf) and m[1:].isfinite().all()
+    # the other pairs: m is 0 but for lp's 32 bits in refp, below 1e-3 beside rows of 1e5 (u |lp| of three rows, times 0.1)
+    assert abs(float(loss) - math.log(2) * (P - 1) / P) < 1e-3 * math.log(2)
+    pair = torch.zeros(6 * P, dtype=torch.bool, device="cuda")
+    pair[0:3] = pair[3 * P:3 * P + 3] = True
+    assert grad.isfinite().all() and not grad[pair].any() and grad[~pair].any()
