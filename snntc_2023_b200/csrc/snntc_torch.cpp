@@ -4,7 +4,8 @@
 // What bounds it: a call on a small problem is a few kernels of some microseconds each, and the same steps written in
 // Python (tensor checks, numpy parameter vectors, a device context manager, torch.empty, a ctypes call with fifteen
 // arguments, a Python autograd.Function) cost 35 to 50 us per operator and direction -- more than its kernels. Nothing
-// is computed here and nothing is kept between calls; the kernels are reached through the C ABI of libsnntc_b200.so.
+// is computed here, and nothing is kept between calls but what an autograd node holds from its forward to its backward (a policy loss:
+// the gradient itself); the kernels are reached through the C ABI of libsnntc_b200.so.
 #include <torch/extension.h>
 
 #include <ATen/cuda/CUDAContext.h>
@@ -548,6 +549,17 @@ Tensor constraint_cost(const std::vector<Tensor>& weights, double K, double K2) 
 }
 
 // ------------------------------------------------------------------------------------------------ embedding, losses on choices
+// The capture that the tensor's current stream is part of; 0: none
+unsigned long long capture_of(const Tensor& t) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(at::cuda::getCurrentCUDAStream(t.get_device()).stream(), &status, &id) != cudaSuccess) {
+    (void)cudaGetLastError();     // (the legacy stream beside another thread's capture: not this call's to report)
+    return 0;
+  }
+  return status == cudaStreamCaptureStatusNone ? 0 : id;
+}
+
 // The nodes below compute gradients by kernels that nothing differentiates: asked for a graph of the gradient they refuse, instead
 // of handing out one that is a constant. And a leaf whose gradient accumulator lives on the default stream -- a graph of the same
 // leaf that was built there is still alive -- would draw that stream, which nothing can capture, into a capture under way, which ends
@@ -556,13 +568,7 @@ Tensor constraint_cost(const std::vector<Tensor>& weights, double K, double K2) 
 void check_backward(const Tensor& on, const char* what) {
   using torch::autograd::Node;
   if (at::GradMode::is_enabled()) throw SnntcFailure(std::string(what) + ": the gradient cannot be differentiated again (create_graph)");
-  const auto current = at::cuda::getCurrentCUDAStream(on.get_device());
-  cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(current.stream(), &capturing) != cudaSuccess) {
-    (void)cudaGetLastError();     // (the legacy stream beside another thread's capture: not this call's to report)
-    return;
-  }
-  if (capturing == cudaStreamCaptureStatusNone) return;
+  if (capture_of(on) == 0) return;
   const auto* wanted = torch::autograd::get_current_graph_task_exec_info();     // empty: all nodes run
   const auto foreign = at::cuda::getDefaultCUDAStream(on.get_device()).unwrap();
   std::vector<Node*> todo = {torch::autograd::get_current_node().get()};
@@ -781,11 +787,14 @@ ChoiceLoss choice_loss_call(const ChoiceState& s, bool grad) {
   return o;
 }
 
-// The gradient that a policy loss formed with its value. The first backward hands it out, scaled by the incoming gradient; autograd
-// may add to it in place or keep it as somebody's .grad, so a second backward over the same graph forms one of its own.
+// The gradient that a policy loss formed with its value. The first backward hands it out, scaled in place by the incoming gradient; autograd
+// may add to it in place or keep it as somebody's .grad, so a second backward over the same graph forms one of its own. And so does one
+// that is not of the forward's capture: replays of a captured backward alone would scale what the last one has scaled, and an eager
+// backward of a captured forward would hand out what the next replay writes.
 struct KeptGradient : torch::CustomClassHolder {
   std::mutex mutex;
   Tensor dz;
+  unsigned long long capture = 0;     // in which it was formed
 };
 
 struct ChoiceLossFunction : torch::autograd::Function<ChoiceLossFunction> {
@@ -793,6 +802,7 @@ struct ChoiceLossFunction : torch::autograd::Function<ChoiceLossFunction> {
     const ChoiceLoss o = choice_loss_call(*s, true);
     auto k = c10::make_intrusive<KeptGradient>();
     k->dz = o.dz;
+    k->capture = capture_of(s->rows.z);
     ctx->save_for_backward({s->rows.z, s->rows.label, o.kept});
     ctx->saved_data["pairs"] = (int64_t)s->P;
     ctx->saved_data["gradient"] = c10::IValue::make_capsule(k);
@@ -810,7 +820,7 @@ struct ChoiceLossFunction : torch::autograd::Function<ChoiceLossFunction> {
     Tensor dz;
     {
       const std::lock_guard<std::mutex> lock(k->mutex);
-      std::swap(dz, k->dz);
+      if (capture_of(saved[0]) == k->capture) std::swap(dz, k->dz);
     }
     if (!dz.defined()) {
       const int64_t R = saved[1].numel();

@@ -684,3 +684,102 @@ def test_a_margin_without_bounds_beside_a_smoothing_of_nothing(P, smoothing):
     pair = torch.zeros(6 * P, dtype=torch.bool, device="cuda")
     pair[0:3] = pair[3 * P:3 * P + 3] = True
     assert grad.isfinite().all() and not grad[pair].any() and grad[~pair].any()
+
+
+def _one_loss(kind, z, lab, old, adv, refp, starts):
+    from snntc_2023_b200 import train
+    if kind == "policy":
+        return train.policy_loss(z, lab, old, adv, ref_logp=refp, kl_coef=0.1)
+    return train.preference_loss(z, lab, starts, beta=0.01) if kind == "preference" else train.label_log_probs(z, lab).sum()
+
+
+def _check_one_loss(kind, grad, z, lab, old, adv, refp, starts):
+    import torch
+    ref = Ref(z.detach(), lab)
+    if kind == "policy":
+        want = _policy_ref(ref, old, adv, refp, 0.2, 0.2, 0.1)
+    elif kind == "preference":
+        want = _preference_ref(ref, starts, None, 0.01, 0.0)
+    else:
+        want = dict(factor=torch.ones_like(ref.lp), factor_tol=torch.zeros_like(ref.lp))
+    ref.check_grad(grad, want["factor"], want["factor_tol"])
+
+
+def _one_loss_inputs(R, J, seed):
+    """Ratios at exp(+-0.1), inside the clip."""
+    import torch
+    z, lab = _logits(R, J, seed)
+    g = torch.Generator("cuda").manual_seed(seed)
+    lp = Ref(z, lab).lp
+    old = (lp + 0.1 * torch.randn(R, device="cuda", generator=g).sign()).float()
+    starts = torch.tensor([0, R // 4 + seed % 2, R // 2, R // 2 + 1, R - 1], device="cuda")
+    return [z, lab, old, torch.randn(R, device="cuda", generator=g), (lp + 0.1).float(), starts]
+
+
+@pytest.mark.parametrize("R,J", [(64, 10), (300, 500), (40, 20011)])
+@pytest.mark.parametrize("kind", ["policy", "preference", "logp"])
+def test_forward_and_backward_captured_apart(R, J, kind):
+    """Two graphs, the backward's replayed again and again behind one replay of the forward's, with other upstream gradients: each
+    replay the gradient at the inputs of the last forward."""
+    import torch
+    sets = [_one_loss_inputs(R, J, 80 + k) for k in range(2)]
+    up = torch.ones((), device="cuda")
+    own = [t.clone() for t in sets[0]]
+    own[0].requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(_one_loss(kind, *own), own[0], up)
+    torch.cuda.synchronize()
+    forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(forward, stream=side):
+        loss = _one_loss(kind, *own)
+    with torch.cuda.graph(backward, stream=side, pool=forward.pool()):
+        (grad,) = torch.autograd.grad(loss, own[0], up, retain_graph=True)
+
+    def replay(k):
+        for dst, src in zip(own, sets[k]):
+            dst.data.copy_(src)                       # (not autograd's to notice: the forward's replay follows)
+        forward.replay()
+
+    for k in (1, 0):
+        replay(k)
+        for u in (-2.0, 0.0, 1.0, 4.0, 4.0):          # (powers of two move no rounding)
+            up.fill_(u)
+            backward.replay()
+            if u == 0:
+                assert not grad.any()
+            else:
+                _check_one_loss(kind, grad / u, *sets[k])
+    torch.cuda.synchronize()
+    # and an eager backward of the captured forward: a tensor of its own, which later replays leave alone
+    with torch.cuda.stream(side):
+        (mine,) = torch.autograd.grad(loss, own[0], up, retain_graph=True)
+    torch.cuda.synchronize()
+    replay(1)
+    backward.replay()
+    _check_one_loss(kind, mine / 4.0, *sets[0])
+    _check_one_loss(kind, grad / 4.0, *sets[1])
+
+
+def test_a_captured_backward_of_an_eager_loss():
+    """The forward ran eagerly, on the stream that the backward is captured on."""
+    import torch
+    own = _one_loss_inputs(50, 30, 5)
+    z = own[0].clone().requires_grad_(True)
+    up = torch.full((), -2.0, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss = _one_loss("policy", z, *own[1:])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        (grad,) = torch.autograd.grad(loss, z, up, retain_graph=True)
+    for u in (-2.0, 4.0, 4.0, 0.0, 1.0):
+        up.fill_(u)
+        graph.replay()
+        if u == 0:
+            assert not grad.any()
+        else:
+            _check_one_loss("policy", grad / u, *own)
