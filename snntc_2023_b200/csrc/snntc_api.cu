@@ -14,7 +14,7 @@ namespace snntc {
 static std::atomic<unsigned long long> g_launches{0};
 static std::atomic<int> g_overlap{1};
 
-// Auxiliary streams: kAuxSlots per device, handed out round robin. The mutex serialises slot creation and every
+// Auxiliary streams: kAuxSlots per device, handed out round robin. The mutex serialises slot creation, the holding of slots and every
 // (record, wait) pair, so that an event is never re-recorded between its record and the wait that refers to it.
 constexpr int kAuxSlots = 4;
 constexpr int kMaxDevices = 64;
@@ -26,11 +26,24 @@ struct AuxPool {
 static std::mutex g_aux_mutex;
 static AuxPool g_aux[kMaxDevices];
 
-AuxSlot* aux_acquire(int overlap_option) {
+// The capture that a stream is part of (0: none), or false where there is no telling or the capture is no longer valid.
+static bool capture_of(cudaStream_t s, unsigned long long* id) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long n = 0;
+  if (cudaStreamGetCaptureInfo(s, &status, &n) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  *id = status == cudaStreamCaptureStatusNone ? 0 : n;
+  return status != cudaStreamCaptureStatusInvalidated;
+}
+
+AuxSlot* aux_acquire(int overlap_option, cudaStream_t caller) {
   const int overlap = overlap_option < 0 ? g_overlap.load(std::memory_order_relaxed) : overlap_option;
   if (!overlap) return nullptr;
   int dev = -1;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return nullptr;
+  unsigned long long mine = 0, its = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices || !capture_of(caller, &mine)) return nullptr;
   std::lock_guard<std::mutex> lock(g_aux_mutex);
   AuxPool& p = g_aux[dev];
   if (p.state == 0) {
@@ -44,13 +57,20 @@ AuxSlot* aux_acquire(int overlap_option) {
     if (!ok) cudaGetLastError();
   }
   if (p.state != 1) return nullptr;
-  return &p.slot[p.next++ % kAuxSlots];
+  for (int k = 0; k < kAuxSlots; ++k) {
+    AuxSlot* a = &p.slot[p.next++ % kAuxSlots];
+    if (a->held || !capture_of(a->stream, &its) || (its != 0 && its != mine)) continue;
+    a->held = true;
+    return a;
+  }
+  return nullptr;
 }
 
 cudaError_t aux_fork(AuxSlot* a, cudaStream_t caller) {
   std::lock_guard<std::mutex> lock(g_aux_mutex);
   cudaError_t e = cudaEventRecord(a->fork, caller);
   if (e == cudaSuccess) e = cudaStreamWaitEvent(a->stream, a->fork, 0);
+  if (e != cudaSuccess) a->held = false;
   return e;
 }
 
@@ -58,6 +78,7 @@ cudaError_t aux_join(AuxSlot* a, cudaStream_t caller) {
   std::lock_guard<std::mutex> lock(g_aux_mutex);
   cudaError_t e = cudaEventRecord(a->join, a->stream);
   if (e == cudaSuccess) e = cudaStreamWaitEvent(caller, a->join, 0);
+  a->held = false;
   return e;
 }
 

@@ -1000,7 +1000,7 @@ int launch_backward(const Geometry& g, const float* grad, const float* x, const 
     if (cudaGetLastError() != cudaSuccess) return E_CUDA;
   }
   // dX and dW only share read-only inputs: run dX on an auxiliary stream beside dW when both are wanted
-  AuxSlot* aux = (dx && parts == 3 && (long)g.R * g.J >= 65536) ? aux_acquire(opt.overlap) : nullptr;
+  AuxSlot* aux = (dx && parts == 3 && (long)g.R * g.J >= 65536) ? aux_acquire(opt.overlap, s) : nullptr;
   cudaStream_t sdx = s;
   if (aux) {
     if (aux_fork(aux, s) != cudaSuccess) return E_CUDA;

@@ -72,16 +72,19 @@ void note_cuda_error(cudaError_t e);
 // A few auxiliary streams per device, each with its own fork/join events, created on first use and kept for
 // the life of the process. Kernels of one call that do not depend on each other (dX and dW) are forked onto
 // one of them and joined back into the caller's stream with events, so the caller still sees ordinary stream
-// order. Slots are handed out round robin; an event record and the wait that refers to it are issued under one
-// lock, so calls from several host threads (or one thread alternating streams) never wait on each other's
-// fork points. aux_acquire returns nullptr when the resources cannot be created or overlap is off: callers then
-// run everything on the one stream.
+// order. Slots are handed out round robin, each to one call at a time: from aux_acquire to aux_join, or to an aux_fork that
+// fails. An event record and the wait that refers to it are issued under one lock, so calls from several host threads (or one
+// thread alternating streams) never wait on each other's fork points. A slot that was forked inside a stream capture
+// stays part of it until the capture ends, well past its join, and work of anything else queued there would end up in that graph
+// or make the capture invalid: such a slot goes to calls of the same capture only. aux_acquire returns nullptr when there is no slot
+// to be had, when the resources cannot be created or when overlap is off: callers then run everything on the one stream.
 struct AuxSlot {
   cudaStream_t stream;
   cudaEvent_t fork;   // recorded on the caller's stream, waited on by the auxiliary stream
   cudaEvent_t join;   // recorded on the auxiliary stream, waited on by the caller's stream
+  bool held;          // by a call between aux_acquire and aux_join
 };
-AuxSlot* aux_acquire(int overlap_option);
+AuxSlot* aux_acquire(int overlap_option, cudaStream_t caller);
 cudaError_t aux_fork(AuxSlot* a, cudaStream_t caller);   // a->stream waits for everything queued on caller so far
 cudaError_t aux_join(AuxSlot* a, cudaStream_t caller);   // caller waits for everything queued on a->stream so far
 

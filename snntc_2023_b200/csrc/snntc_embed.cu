@@ -625,7 +625,7 @@ int snntc_embedding_forward_sort(const void* ids, int id_bytes, const float* tab
   cudaStream_t s = (cudaStream_t)stream, side = s;
   const Ids in{ids, id_bytes == 8, V, padding};
   const SortSpace w(N);
-  snntc::AuxSlot* aux = snntc::aux_acquire(-1);
+  snntc::AuxSlot* aux = snntc::aux_acquire(-1, s);
   if (aux) {
     const cudaError_t e = snntc::aux_fork(aux, s);
     if (e != cudaSuccess) {

@@ -349,3 +349,79 @@ def test_a_capture_beside_a_live_graph_of_a_side_stream():
     graph.replay()
     torch.cuda.synchronize()
     _check(ids, table, up, y.detach(), w.grad, 1.0, False)
+
+
+def test_a_long_lookup_beside_another_thread_s_capture():
+    """While one thread captures long lookups with their gradients -- sorts on the library's streams are then part of its capture --
+    another runs eagerly, and one captures for itself: each has its own results, and the captures are whole."""
+    import contextlib
+    import threading
+    from concurrent.futures import ThreadPoolExecutor
+
+    import torch
+    from snntc_2023_b200 import ops
+    N, V, D = 12_001, 700, 512
+    cases = [_case(N, V, D, 40 + k) for k in range(3)]
+
+    def step(k, times=1):
+        ids, table, up = cases[k]
+        for _ in range(times):
+            w = table.detach().requires_grad_(True)
+            y = ops.snn_embedding(ids, w, spikes=True)
+            out = y.detach(), torch.autograd.grad(y, w, up)[0]
+        return out
+
+    plain = [step(k) for k in range(3)]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    for k, s in enumerate(streams):                   # what the eager calls below allocate is there already
+        with torch.cuda.stream(s):
+            kept = [step(k) for _ in range(6)]
+            del kept
+    torch.cuda.synchronize()
+    inside, finished = threading.Barrier(3, timeout=60), threading.Barrier(3, timeout=60)
+
+    def captured(k):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.stream(streams[k]):
+            try:
+                graph.capture_begin(capture_error_mode="thread_local")
+                out = step(k)
+                inside.wait()                         # both captures have drawn a stream of the library's
+                out = step(k, times=4)
+                finished.wait()
+                graph.capture_end()
+            except BaseException:
+                inside.abort()
+                finished.abort()
+                with contextlib.suppress(RuntimeError):
+                    graph.capture_end()
+                raise
+        return graph, out
+
+    def eager(k):
+        try:
+            inside.wait()
+            with torch.cuda.stream(streams[k]):
+                out = [step(k) for _ in range(6)]
+                streams[k].synchronize()
+            finished.wait()
+        except BaseException:
+            inside.abort()
+            finished.abort()
+            raise
+        return out
+
+    with ThreadPoolExecutor(3) as pool:
+        work = [pool.submit(captured, 0), pool.submit(captured, 1), pool.submit(eager, 2)]
+        results = [f.result() for f in work]
+    same = lambda got, k: torch.equal(got[0], plain[k][0]) and torch.equal(got[1], plain[k][1])  # noqa: E731
+    assert all(same(out, 2) for out in results[2])
+    for k in range(2):
+        graph, out = results[k]
+        for t in out:
+            t.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert same(out, k)
+    assert same(step(2), 2)                           # and the library's streams serve eager calls again
