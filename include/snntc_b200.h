@@ -204,9 +204,10 @@ SNNTC_API int snntc_sgdm_step(float* w, const float* g, float* vel, size_t n, fl
  *                    snntc_embedding_sorted_bytes(N, D) bytes, 256-byte aligned, which the caller keeps until then. Where that is
  *                    0 (a short lookup) it is snntc_embedding_forward, and the backward sorts for itself.
  * snntc_embedding_backward  dtable[V,D] is written in full: the gradient of the table for the upstream gradient g[N,D], each row
- *                    summed over its tokens in the order of t (zeros where no token names it). `table` is read only where
- *                    `spikes` is not 0 and may be null otherwise. `sorted`: what snntc_embedding_forward_sort has left for the same
- *                    ids, padding and V, and ids may be null; or null. The same bits every run, either way.
+ *                    summed over its tokens in 32 bits (zeros where no token names it), in an order that the ids of the call fix:
+ *                    the same call gives the same bits every run, but a row's last bits may go with the call's other tokens. `table`
+ *                    is read only where `spikes` is not 0 and may be null otherwise. `sorted`: what snntc_embedding_forward_sort has
+ *                    left for the same ids, padding and V, and ids may be null; or null. The same bits either way.
  *
  * For the losses z[R,J] are spike values (logits are -z) and labels[R] int64; a row whose label is outside [0, J) does not count:
  * its logits are not read, its log-probability is 0 and its gradient 0. stats_2R (R pairs of floats) receives what the backward

@@ -2,10 +2,10 @@
 //
 //   forward   y[t,:] = scale * E[id_t,:], or exp(scale * E[id_t,:]) where the rows hold spike times (as the input encoding of
 //             snntc_train.cu does for pixels); no_spike where the id is the padding id or outside the table
-//   gradient  dE[v,:] = f * sum over the t with id_t = v of g[t,:], in the order of t; f = scale, or scale * exp(scale * E[v,:])
+//   gradient  dE[v,:] = f * sum over the t with id_t = v of g[t,:]; f = scale, or scale * exp(scale * E[v,:])
 //
 // The gradient sorts (id, position) pairs by id -- a least-significant-digit radix sort, stable, so that every id's positions
-// stay in order -- and sums runs of equal ids. No atomics on floats: the same bits every run.
+// stay in order -- and sums runs of equal ids, cut at places that the ids of the call fix. No atomics on floats: the same bits every run.
 #include "../../include/snntc_b200.h"
 #include "snntc_common.cuh"
 #include "snntc_launch.cuh"
@@ -291,9 +291,13 @@ sort_scatter_kernel(Keys keys, const int* counts, uint2* __restrict__ out, long 
 // ---- sums of runs of equal keys. What bounds them is memory: g read once, the table's gradient written once (131 072 tokens of 512
 // values on as many rows: 537 MB in 92 us, 5.8 TB/s, behind 26 us of sort and before 8 us of joins).
 // The sorted pairs are cut into tiles of M; a group of L lanes takes a tile and L parts of the rows, kTermsAhead rows of g in flight.
-// Runs inside a tile are done there and then; of one that crosses a border the first tile leaves its part in `tail`, the others theirs in
-// `head`, and the joining kernel adds those in order. So a token that every second place holds is summed by as many CTAs as its share,
-// and the order of summation depends on the sizes alone. (One CTA for each run: 8.3 ms, most of it the most frequent token's.)
+// Runs inside a tile are done there and then, in the order of t; of one that crosses a border the first tile leaves its part in `tail`, the
+// others theirs in `head`, and the joining kernel adds those: one after the other, or in eight interleaved sums where there are more than
+// eight. So a token that every second place holds is summed by as many CTAs as its share, in an order that the sorted ids fix: the tokens
+// below it move its borders, and with them its last bits. (One CTA for each run: 8.3 ms, most of it the most frequent token's.)
+// The sums have 32 bits. In 64, parts and joins included, the error of 131 072 tokens of 512 values falls from 1.1e-7 to 2.3e-8 of the
+// gradient's norm (float32's own step is 6e-8), and lookup and gradient take 174 us instead of 167; of 10^6 of 16 on 4096 rows 1.8e-7,
+// 2.6e-8, 141 and 128 us.
 // Rows that no token names are zeroed by further CTAs of the same launch, a warp for 32 rows or a share of them: each lane looks a row up
 // in the sorted keys. (A clearing of the whole table in front would write the named rows twice.)
 constexpr int kTermsAhead = 8;
@@ -402,7 +406,7 @@ __global__ void __launch_bounds__(kThreads) embed_run_sums_kernel(RunSums q) {
 }
 
 // Runs that go on behind the tile in which they begin: a warp looks at a tile and 32 parts, adds a run of a few tiles itself and leaves
-// a longer one to all warps of its CTA, an eighth of the tiles each.
+// a longer one to all warps of its CTA, every eighth of the tiles each, whose sums are then added in the order of the warps.
 template <Kind KIND>
 __global__ void __launch_bounds__(kThreads) embed_join_kernel(RunSums q) {
   chain_wait();

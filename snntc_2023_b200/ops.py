@@ -365,8 +365,8 @@ def snn_embedding(ids, weight, scale=1.0, padding_idx=None, spikes=False, no_spi
     """Rows of `weight` [tokens, D] for integer ids (int32 or int64, any shape): [..., D] of scale * row or, with spikes=True,
     exp(scale * row) -- rows of spike times encoded as train.encode(p, scale, one_minus=False) encodes pixels. Where an id
     is `padding_idx` or outside the table, all D values are `no_spike` and nothing gets a gradient. Differentiable in
-    `weight`: every row's gradient is summed over its tokens in their order, the same bits every run. `grad_sink`: a tensor
-    that receives the gradient instead of autograd, as for the layers: written, not accumulated, so one call of a table in a
-    backward pass. The gradient cannot be differentiated again."""
+    `weight`: every row's gradient is summed over its tokens in 32 bits and an order that the ids of the call fix, so the same
+    call gives the same bits every run. `grad_sink`: a tensor that receives the gradient instead of autograd, as for the layers:
+    written, not accumulated, so one call of a table in a backward pass. The gradient cannot be differentiated again."""
     return _lib.native().embedding(_tensor(ids, "ids"), _tensor(weight, "weight"), float(scale), bool(spikes), padding_idx,
                                    float(no_spike), grad_sink)
