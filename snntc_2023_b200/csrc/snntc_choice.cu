@@ -35,6 +35,9 @@ using snntc::streaming;
 __device__ __forceinline__ bool counts(long long label, int J) { return label >= 0 && label < J; }
 
 // exp(d) for d <= 0 as 2^(d log2 e), one product and one instruction: off by 2^-22 + |d| 2^-23 relative, and by some -5e-8 in the mean.
+// With expf in its place the gradients' largest relative errors fall from 23 half steps of float32 to 14 (spike values up to some 13
+// apart), their norm's stays at one, and it is the dearer one: policy loss with gradient of 8192 rows of 50 021 598 us instead of 577, of
+// 32 768 of 1500 95, 87; log-probabilities with gradient of 4096 of 16 384 131, 125.
 __device__ __forceinline__ float exp_term(float d) {
   float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * 1.44269504f));
@@ -432,7 +435,7 @@ __device__ __forceinline__ float row_numbers(const float* z, const long long* la
 template <int T, int G, int NV, bool HOLD, bool POLICY>
 __device__ __forceinline__ void rows_of_cta(const float* z, const long long* labels, const RowOut& out, const Policy& pol, long long R, int J,
                                             long long blk, double3* term) {
-  static_assert(G <= 32 || G == T, "a row belongs to part of a warp, a warp or the CTA");
+  static_assert(G <= 32 || (G == T && !HOLD), "a row belongs to part of a warp, a warp or, streamed, the CTA");
   constexpr int kRows = T / G, W = G < 32 ? G : 32, kGradAhead = NV == 8 ? 8 : 2;
   __shared__ float2 stats[kRows > T / 32 ? kRows : T / 32];   // (top, total): of rows, or of a row's warps
   __shared__ float factors[kRows];
@@ -452,7 +455,7 @@ __device__ __forceinline__ void rows_of_cta(const float* z, const long long* lab
 
   RowValues<NV> v;
   Ends e(row, J, gl);
-  float top = -FLT_MAX, total = 0.f;
+  float top = -FLT_MAX, total = 0.f, over = 0.f;
   if constexpr (HOLD) {
     v = load_row<NV>(row, J, live, gl, G);
     float m[4] = {-FLT_MAX, -FLT_MAX, -FLT_MAX, -FLT_MAX}, s[4] = {};
@@ -465,6 +468,7 @@ __device__ __forceinline__ void rows_of_cta(const float* z, const long long* lab
       s[k % 4] += v.x[k];
     }
     total = lanes_sum<W>((s[0] + s[1]) + (s[2] + s[3]));
+    over = 1.f / total;                        // (here, not behind the barrier: 16 384 rows of 1000 41.0 us, 42.3)
   } else {
     if (live) {
       int v0 = gl;
@@ -484,7 +488,6 @@ __device__ __forceinline__ void rows_of_cta(const float* z, const long long* lab
     total = lanes_sum<W>(total * expf(top - t));
     top = t;
   }
-  const float held_top = top;                  // what the held values are relative to
   if (G == T) {
     if (lane == 0) stats[tid >> 5] = make_float2(top, total);
     __syncthreads();
@@ -508,7 +511,7 @@ __device__ __forceinline__ void rows_of_cta(const float* z, const long long* lab
   const float f = factors[own];
   if constexpr (HOLD) {
     float* to = pol.dz + r * J;
-    const float scale = f * (expf(held_top - top) / total);
+    const float scale = f * over;
 #pragma unroll
     for (int k = 0; k < 4 * NV; ++k) v.x[k] = f == 0.f ? 0.f : v.x[k] * scale;
     store_row<NV>(to, row, v, J, label, f, gl, G);
