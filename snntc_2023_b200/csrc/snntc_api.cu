@@ -3,6 +3,7 @@
 // translation of the `params` vectors into a Geometry, and dispatch to the kernel launchers.
 #include "../../include/snntc_b200.h"
 #include "snntc_common.cuh"
+#include "snntc_launch.cuh"
 
 #include <limits.h>
 #include <string.h>
@@ -90,6 +91,13 @@ void note_cuda_error(cudaError_t e) {
   if (e == cudaSuccess) return;
   strncpy(g_cuda_err, cudaGetErrorString(e), sizeof(g_cuda_err) - 1);
   g_cuda_err[sizeof(g_cuda_err) - 1] = 0;
+}
+
+int done() {
+  count_launch();
+  const cudaError_t e = cudaGetLastError();
+  note_cuda_error(e);
+  return e == cudaSuccess ? SNNTC_OK : SNNTC_E_CUDA;
 }
 }  // namespace snntc
 

@@ -20,13 +20,12 @@
 
 #include <utility>
 
-namespace snntc { void count_launch(int n = 1); void note_cuda_error(cudaError_t e); }
-
 namespace {
 
 namespace cg = cooperative_groups;
 using snntc::chain_next;
 using snntc::chain_wait;
+using snntc::done;
 using snntc::launch_chained;
 using snntc::ld_plain;
 using snntc::ld_stream_at;
@@ -663,14 +662,6 @@ __global__ void __launch_bounds__(512) mean_kernel(const double* terms, int n, f
   for (int k = threadIdx.x; k < n; k += blockDim.x) s.x += ld_plain(terms + k);
   s = block_sum(s);
   if (threadIdx.x == 0) *mean = (float)(s.x / n);
-}
-
-int done() {
-  snntc::count_launch();
-  const cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) return SNNTC_OK;
-  snntc::note_cuda_error(e);
-  return SNNTC_E_CUDA;
 }
 
 int check_rows(long long R, int J) {

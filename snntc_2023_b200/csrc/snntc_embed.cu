@@ -17,6 +17,7 @@ namespace {
 
 using snntc::chain_next;
 using snntc::chain_wait;
+using snntc::done;
 using snntc::launch_chained;
 using snntc::ld_plain;
 using snntc::ld_stream;
@@ -466,14 +467,6 @@ __global__ void __launch_bounds__(kThreads) embed_join_kernel(RunSums q) {
     }
     __syncthreads();
   }
-}
-
-int done() {
-  snntc::count_launch();
-  const cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess) return SNNTC_OK;
-  snntc::note_cuda_error(e);
-  return SNNTC_E_CUDA;
 }
 
 int check_sizes(int id_bytes, long long N, long long V, int D) {

@@ -109,6 +109,9 @@ cudaError_t launch_chained(void (*kernel)(Params...), ChainGrid where, dim3 bloc
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
+// Counts a launch that has just been made: SNNTC_OK, or SNNTC_E_CUDA with its error noted for snntc_last_cuda_error.
+int done();
+
 // Raises the kernel's limit of dynamic shared memory on the current device to at least `bytes`; a call into the runtime only
 // when it grows. What every kernel may have anyway (48 KB less its static arrays, which are below 16 KB in all that ask here) is not
 // looked up.
