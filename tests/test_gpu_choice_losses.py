@@ -783,3 +783,68 @@ def test_a_captured_backward_of_an_eager_loss():
             assert not grad.any()
         else:
             _check_one_loss("policy", grad / u, *own)
+
+
+# Row lengths and counts that the shapes above leave out: rows streamed by a warp (1025 to 1800 outputs), parts of a warp to a row with more
+# rows than one cluster takes, and two turns of the one cluster (9 to 16 CTAs' worth of rows).
+MORE_SHAPES = [(40, 1500), (3000, 1501), (7, 1800), (300, 1025), (2000, 60), (2000, 120), (600, 250), (200, 500), (100, 500), (3000, 10), (700, 50),
+               (20000, 30)]
+
+
+@pytest.mark.parametrize("R,J", MORE_SHAPES)
+def test_label_log_probs_of_more_shapes(R, J):
+    test_label_log_probs_and_their_gradient(R, J)
+
+
+@pytest.mark.parametrize("R,J", MORE_SHAPES)
+def test_policy_loss_of_more_shapes(R, J):
+    """Ratios at exp(+-0.1) and, beyond the clip, at exp(+-0.5)."""
+    import torch
+    from snntc_2023_b200 import train
+    z, lab = _logits(R, J, R + 5 * J)
+    ref = Ref(z, lab)
+    g = torch.Generator("cuda").manual_seed(9)
+    off = torch.tensor([-0.5, -0.1, 0.1, 0.5], device="cuda")[torch.randint(0, 4, (R,), device="cuda", generator=g)]
+    old, adv, refp = (ref.lp + off).float(), torch.randn(R, device="cuda", generator=g), (ref.lp + 0.5 * torch.randn(R, device="cuda", generator=g)).float()
+    want = _policy_ref(ref, old, adv, refp, 0.2, 0.25, 0.3)
+    assert not want["near"]
+    z1 = z.clone().requires_grad_(True)
+    loss, stats = train.policy_loss(z1, lab, old, adv, ref_logp=refp, clip_low=0.2, clip_high=0.25, kl_coef=0.3, with_stats=True)
+    for got, name in ((loss.detach(), "loss"), (stats[0], "kl")):
+        assert abs(float(got) - want[name]) <= want[name + "_tol"] + abs(want[name]) * U
+    assert abs(float(stats[1]) - want["clipped"]) <= U
+    for _ in range(2):                                # the gradient that was formed with the loss, and one formed from what it keeps
+        (grad,) = torch.autograd.grad(loss, z1, retain_graph=True)
+        ref.check_grad(grad, want["factor"], want["factor_tol"])
+
+
+@pytest.mark.parametrize("R,J", MORE_SHAPES)
+def test_preference_loss_of_more_shapes(R, J):
+    for with_ref in (True, False):
+        test_preference_loss_and_its_gradient(R, J, 3, 2, with_ref)
+
+
+def test_two_threads_and_their_errors():
+    """As test_two_threads_at_once, with an error in a thread as an error of the test, and every round counted."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    import torch
+    cases = []
+    for k, (R, J) in enumerate(((300, 40), (64, 9000))):
+        z, lab = _logits(R, J, 70 + k)
+        cases.append((z, lab, -2 - torch.rand(R, device="cuda"), torch.randn(R, device="cuda"), -2 - torch.rand(R, device="cuda"),
+                      torch.tensor([0, R // 4, R // 2, R // 2, R], device="cuda")))
+    plain = [_all_losses(c[0].clone().requires_grad_(True), *c[1:]) for c in cases]
+    torch.cuda.synchronize()
+
+    def work(k):
+        equal = 0
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = _all_losses(cases[k][0].clone().requires_grad_(True), *cases[k][1:])
+                torch.cuda.current_stream().synchronize()
+                equal += len(got) == len(plain[k]) and all(torch.equal(a, b) for a, b in zip(got, plain[k]))
+        return equal
+
+    with ThreadPoolExecutor(2) as pool:
+        assert list(pool.map(work, range(2))) == [20, 20]

@@ -425,3 +425,51 @@ def test_a_long_lookup_beside_another_thread_s_capture():
         torch.cuda.synchronize()
         assert same(out, k)
     assert same(step(2), 2)                           # and the library's streams serve eager calls again
+
+
+@pytest.mark.parametrize("bits", [32, 64])
+@pytest.mark.parametrize("spikes", [False, True])
+def test_a_sink_behind_the_sort_beside_the_lookup(bits, spikes):
+    """A long lookup in training, whose tokens are sorted beside it, with the gradient into a sink: the bits that autograd would hand
+    out, nothing of what the sink held, nothing for autograd."""
+    import torch
+    from snntc_2023_b200 import ops
+    ids, table, up = _case(12_001, 700, 512, 17, torch.int32 if bits == 32 else torch.int64, skew=True)
+    ids[::9] = -1
+    w = table.clone().requires_grad_(True)
+    (want,) = torch.autograd.grad(ops.snn_embedding(ids, w, scale=0.5, spikes=spikes), w, up)
+    sink = torch.full_like(table, float("nan"))
+    for _ in range(2):
+        y = ops.snn_embedding(ids, w, scale=0.5, spikes=spikes, grad_sink=sink)
+        y.backward(up)
+        assert torch.equal(sink, want) and w.grad is None
+    _check(ids, table, up, y.detach(), sink, 0.5, spikes)
+
+
+def test_two_threads_and_their_errors():
+    """As test_two_threads_at_once, with an error in a thread as an error of the test, and every round counted."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    import torch
+    from snntc_2023_b200 import ops
+    cases = [_case(12_000, 3000, 400, 1), _case(500, 90, 33, 2)]
+
+    def call(ids, table, up):
+        w = table.clone().requires_grad_(True)
+        y = ops.snn_embedding(ids, w, spikes=True)
+        return y.detach(), torch.autograd.grad(y, w, up)[0]
+
+    plain = [call(*c) for c in cases]
+    torch.cuda.synchronize()
+
+    def work(k):
+        equal = 0
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got = call(*cases[k])
+                torch.cuda.current_stream().synchronize()
+                equal += all(torch.equal(a, b) for a, b in zip(got, plain[k]))
+        return equal
+
+    with ThreadPoolExecutor(2) as pool:
+        assert list(pool.map(work, range(2))) == [20, 20]
