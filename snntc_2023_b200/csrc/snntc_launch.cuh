@@ -18,8 +18,12 @@ namespace snntc {
 // 64 SMs: the whole layer 1119 -> 1278 us), and has nothing to gain from 1.5 us.
 constexpr long kChainThreads = 148L * 128;
 // A kernel that streams -- CTAs of equal work, each with its own stretch -- asks for it as streaming(grid) and has it from a wave of full
-// SMs on, too: its later CTAs go wherever an SM is free, which evens out how the first ones were placed. Passes one behind the other: a
-// lookup of 20 000 rows of 300 values 10.4 -> 7.6 us, of 65 536 of 512 30.8 -> 28.5, log-probabilities of 4096 rows of 32 768 78.2 -> 75.8.
+// SMs on, too: its later CTAs go wherever an SM is free, which evens out how the first ones were placed. One behind the other in a graph,
+// over inputs beyond L2: a lookup of 20 000 rows of 300 values in random order 11.9 -> 11.3 us, of 65 536 of 512 41.1 -> 40.5,
+// log-probabilities of 16 384 rows of 1000 14.6 -> 14.1, of 4096 of 32 768 82 -> 80.7, with the policy loss's gradient 178.8 -> 178.3.
+// Grids between the two limits stay in plain order: most would gain, too (lookup of 4000 rows of 300 5.4 -> 4.9, of 8000 6.7 -> 6.2, policy
+// loss of 2000 of 300 12.4 -> 11.5), but grids of few and long CTAs crowd (log-probabilities of 300 rows of 32 768 10.9 -> 11.5), and what
+// they cost behind other kernels is not measured.
 // (Not for kernels behind a sort or sums of unequal tiles: the gradient of 9000 tokens of 768 values 32.5 -> 36.3.)
 constexpr long kStreamThreads = 148L * 2048;
 __device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
