@@ -73,7 +73,7 @@ __device__ __forceinline__ PolicyRow policy_row(double lp, double old, double ad
   p.loss = -(p.clipped ? (adv > 0 ? q.upper : q.lower) * adv : unclipped);
   if (has_ref) {
     const double away = ref - lp, e = expm1(away);
-    p.kl = e - away;
+    p.kl = isinf(e) ? e : e - away;              // (away is infinite, too, where an output at +inf rules the label out)
     if (q.kl_coef != 0) {        // (a label that does not spike overflows e: without a weight that stays out of the loss)
       p.slope -= q.kl_coef * e;
       p.loss += q.kl_coef * p.kl;

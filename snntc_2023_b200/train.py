@@ -59,7 +59,8 @@ def policy_loss(logit, label, old_logp, advantage, ref_logp=None, clip_low=0.2, 
     logit [..., classes]; label, old_logp, advantage, ref_logp [...], one value per row, the last three constants. with_stats=True
     also returns [mean k, share of rows whose ratio was clipped]; with kl_coef = 0 k has no part in loss and gradient. Where k
     overflows -- a label that does not spike, lp near -1e5, beside a reference of -3 -- the mean k is infinite, and with kl_coef > 0
-    the loss is, too, and that row's gradient (already from ref_logp - lp = 88 on, float32's range) infinite or NaN. The gradient is formed with the loss, in the pass that reads the
+    the loss is, too, and that row's gradient (already from ref_logp - lp = 88 on, float32's range) infinite or NaN; a ratio that
+    overflows beside a negative advantage does the same. The gradient is formed with the loss, in the pass that reads the
     logits; it cannot be differentiated again."""
     loss, stats = _lib.native().policy_loss(_tensor(logit, "logit"), _tensor(label, "label"), _tensor(old_logp, "old_logp"),
                                             _tensor(advantage, "advantage"),

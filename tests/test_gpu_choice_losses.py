@@ -848,3 +848,19 @@ def test_two_threads_and_their_errors():
 
     with ThreadPoolExecutor(2) as pool:
         assert list(pool.map(work, range(2))) == [20, 20]
+
+
+@pytest.mark.parametrize("R,J", SILENT)
+def test_a_label_that_its_network_rules_out(R, J):
+    """The label's output at +inf: its ratio is 0, its KL term infinite, which is the mean's; the loss without a weight for it is finite,
+    and with one infinite, no NaN."""
+    import torch
+    from snntc_2023_b200 import train
+    z, lab, old, adv, refp, at = _beside_a_silent_label(R, J, R + J + 2)
+    z[at, lab[at]] = math.inf
+    old[at], adv[at] = -2.0, 1.0
+    z1 = z.clone().requires_grad_(True)
+    loss, stats = train.policy_loss(z1, lab, old, adv, ref_logp=refp, with_stats=True)
+    (grad,) = torch.autograd.grad(loss, z1)
+    assert loss.isfinite() and float(stats[0]) == math.inf and grad.isfinite().all() and not grad[at].any()
+    assert float(train.policy_loss(z, lab, old, adv, ref_logp=refp, kl_coef=0.1)) == math.inf
